@@ -16,31 +16,13 @@
 #include <cfloat>
 
 #include "b200_common.cuh"
+#include "b200_philox.cuh"
 
 namespace b200 {
 
-// ---------------- Philox-4x32-10 (Salmon et al., SC'11) ----------------
-__host__ __device__ __forceinline__ void philox_round(uint32_t c[4], uint32_t k[2]) {
-  const uint64_t p0 = (uint64_t)0xD2511F53u * c[0];
-  const uint64_t p1 = (uint64_t)0xCD9E8D57u * c[2];
-  const uint32_t hi0 = (uint32_t)(p0 >> 32), lo0 = (uint32_t)p0;
-  const uint32_t hi1 = (uint32_t)(p1 >> 32), lo1 = (uint32_t)p1;
-  const uint32_t n0 = hi1 ^ c[1] ^ k[0];
-  const uint32_t n2 = hi0 ^ c[3] ^ k[1];
-  c[0] = n0;
-  c[1] = lo1;
-  c[2] = n2;
-  c[3] = lo0;
-}
 __host__ __device__ __forceinline__ uint32_t philox_u32(uint64_t key, uint64_t step, uint32_t idx) {
   uint32_t c[4] = {idx, (uint32_t)step, (uint32_t)(step >> 32), 0x42323030u};
-  uint32_t k[2] = {(uint32_t)key, (uint32_t)(key >> 32)};
-#pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    philox_round(c, k);
-    k[0] += 0x9E3779B9u;
-    k[1] += 0xBB67AE85u;
-  }
+  philox_4x32_10(c, key);
   return c[0];
 }
 // Uniform in (0, 1) from the top 24 bits.

@@ -285,6 +285,17 @@ def philox_u32(key: int, step: int, idx: np.ndarray) -> np.ndarray:
     return c0.astype(np.uint32)
 
 
+def philox_4x32(counter, key: int) -> list[np.ndarray]:
+    """Philox-4x32-10 of four broadcastable uint32 counter words: its four output words."""
+    c0, c1, c2, c3 = (np.asarray(c, dtype=np.uint64) & _MASK32 for c in counter)
+    k0, k1 = np.uint64(key & 0xFFFFFFFF), np.uint64((key >> 32) & 0xFFFFFFFF)
+    for _ in range(10):
+        p0, p1 = _M0 * c0, _M1 * c2
+        c0, c1, c2, c3 = (p1 >> np.uint64(32)) ^ c1 ^ k0, p1 & _MASK32, (p0 >> np.uint64(32)) ^ c3 ^ k1, p0 & _MASK32
+        k0, k1 = (k0 + _W0) & _MASK32, (k1 + _W1) & _MASK32
+    return [c.astype(np.uint32) for c in np.broadcast_arrays(c0, c1, c2, c3)]
+
+
 def philox_uniform(key: int, step: int, idx: np.ndarray) -> np.ndarray:
     x = philox_u32(key, step, idx)
     return ((x >> 8).astype(np.float32) + np.float32(0.5)) * np.float32(1.0 / 16777216.0)
@@ -507,3 +518,51 @@ def xielu_ref(x, params):
     xf = x.float()
     y = torch.where(xf > 0, ap * xf * xf + beta * xf, an * torch.expm1(torch.minimum(xf, eps)) - an * xf + beta * xf)
     return y.to(x.dtype)
+
+
+# --------------------------------------------------------------------------
+# training ops
+# --------------------------------------------------------------------------
+def dropout_cut(p: float) -> int:
+    """Elements whose 16 random bits are below this are dropped."""
+    return int(p * 65536 + 0.5)
+
+
+def dropout_scale(cut: int) -> float:
+    """What kept elements are multiplied by: 1 / (1 - cut / 65536)."""
+    return 65536.0 / (65536 - cut) if cut < 65536 else 0.0
+
+
+def dropout_keep_ref(rows: int, K: int, p: float, seed: int, offset: int = 0) -> torch.Tensor:
+    """The mask [rows, K] of :func:`ops.dropout`: one Philox block for eight
+    neighbouring columns, 16 bits each, the low half of a word first."""
+    blocks = (K + 7) // 8
+    words = philox_4x32((np.arange(blocks)[None, :], np.arange(rows)[:, None], offset & 0xFFFFFFFF, offset >> 32), seed)
+    bits = np.stack([h for w in words for h in (w & np.uint32(0xFFFF), w >> np.uint32(16))], -1)
+    return torch.from_numpy(bits.reshape(rows, blocks * 8)[:, :K] >= dropout_cut(p))
+
+
+def dropout_ref(x, p, seed, offset=0, residual=None):
+    K = x.shape[-1] if x.dim() else 1
+    rows = x.numel() // K if K else 0
+    keep = dropout_keep_ref(rows, K, p, seed, offset).reshape(x.shape).to(x.device)
+    y = torch.where(keep, x.float() * dropout_scale(dropout_cut(p)), torch.zeros((), device=x.device))
+    if residual is not None:
+        y = y + residual.float()
+    return y.to(x.dtype)
+
+
+def block_norms_ref(x, delta, post_w, pre_w, eps, gate=None, scale=1.0, offset_one=False, round_branch=False):
+    """(y, h) of :func:`ops.block_norms`; differentiable."""
+    one = 1.0 if offset_one else 0.0
+
+    def rms(v, w):
+        return v * torch.rsqrt(v.pow(2).mean(-1, keepdim=True) + eps) * (w.float() + one)
+
+    u = delta.float() if post_w is None else rms(delta.float(), post_w)
+    if round_branch:
+        u = u.to(x.dtype).float()
+    if gate is not None:
+        u = u * gate.float()
+    y = (x.float() + scale * u).to(x.dtype)
+    return y, None if pre_w is None else rms(y.float(), pre_w).to(x.dtype)
