@@ -703,6 +703,10 @@ bool make_tmap_2d_sw(CUtensorMap* out, const void* ptr, int64_t rows, int64_t co
   }
   auto enc = get_encode_fn();
   if (!enc) return false;
+  // the driver call needs a context of the calling thread, which a thread that has made
+  // no launch yet (autograd's) does not have
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return false;
   CUtensorMapDataType dt = dtype_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                            : dtype_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;

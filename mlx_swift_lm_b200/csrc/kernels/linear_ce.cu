@@ -1,0 +1,678 @@
+// Softmax cross entropy of a linear head, without the logits:
+//
+//   u = h . W^T,  z = cap > 0 ? cap * tanh(u / cap) : u          (T x V, never stored)
+//   d = log sum_{v != y} exp z_v - z_y,  loss = log(1 + exp d)
+//   G[t, v] = dloss_t * (p_v - [v = y]) * dz/du,  p_v = exp(z_v - z_y - loss)
+//   dh = G . W,  dW = G^T . h
+//
+// The target's logit stands apart from the sum over the others, so a loss near
+// zero (and p_y - 1 = expm1(-loss)) keeps its digits. It is a dot product in
+// fp32 of its own; the others come from the tensor cores.
+//
+// Forward: one product whose tiles leave a (max, sum of exp) pair per row and
+// 256 columns. Backward: the vocabulary in pieces; each forms its logits again
+// and turns them into G in bf16 (at most 2^-8 of each entry, as any bf16 product
+// of gradients rounds its operands), which two products with fp32 accumulators
+// contract with W and h. So the work is 2 T V K forward and 6 backward, 4 of
+// them the gradients' own; the memory is one piece of G.
+//
+// Only scored rows take part: they are gathered first (stable order) and their
+// count stays on the device, so padding costs nothing and whatever ignored rows
+// hold (NaN included) reaches no gradient.
+//
+// One kernel does the four products (Op): persistent CTAs, one per SM, walk 128 x
+// 256 output tiles. Warp 0 fetches operands by TMA into a ring of 64-deep stages,
+// warp 1 issues tcgen05.mma into one of two accumulators in tensor memory (2 x
+// 256 columns), warps 4 - 7 work on the other one's finished tile, a row of it
+// per thread: the softmax arithmetic runs under the next tile's product.
+#include "b200_common.cuh"
+
+namespace b200 {
+
+bool make_tmap_2d(CUtensorMap* out, const void* ptr, int64_t rows, int64_t cols, int64_t ld_elems, int box_rows,
+                  int box_cols, int dtype_bytes);
+
+namespace lce {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+enum Op : int {
+  kStats = 0,  // A = h rows, B = W rows; out: (max, sum exp) of each row's 256 columns
+  kGrad = 1,   // A = h rows, B = W rows of a piece; out: G
+  kDh = 2,     // A = G (vocabulary inner), B = W columns; out: fp32 dh, added piece by piece
+  kDw = 3,     // A = G columns, B = h columns (rows contracted); out: bf16 dW
+};
+
+struct Args {
+  const int* count;      // [1] scored rows n
+  const int* target;     // [T] target of each scored row (-1: out of range)
+  const int* token;      // [T] the scored row's index in the batch
+  const float* zt;       // [T] target logits (capped)
+  const float* loss;     // [T] losses of the scored rows
+  const float* dloss;    // incoming gradient, element token * dloss_stride
+  int64_t dloss_stride;
+  int mean;              // dloss is of the mean: divide by n
+  float2* part;          // kStats: [tiles of 256 columns][T]
+  __nv_bfloat16* G;      // [T][ldg]
+  int64_t ldg;
+  float* acc;            // kDh: [splits][T][K]
+  __nv_bfloat16* dw;     // kDw: [V][K]
+  int64_t lddw;
+  int T, V, K;
+  int v0, nv;            // the piece's first column and columns
+  int splits, first;     // kDh: parts of the contraction; first piece stores, others add
+  float cap, inv_cap;    // cap 0: none
+};
+
+constexpr int kTileM = 128, kTileN = 256, kStages = 4;
+constexpr int kABytes = kTileM * 128, kBBytes = kTileN * 128, kStageBytes = kABytes + kBBytes;
+constexpr int kBars = 2 * kStages + 4;
+constexpr int kSmem = kStages * kStageBytes + kBars * 8 + 16 + 1024;
+constexpr int kThreads = 256;
+constexpr int kGroupM = 16;  // row tiles walked per column tile before the next: W is read once per 16 x 128 rows, h stays in L2
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The tile walk of one launch: `mt` x `nt` tiles (times `splits` of the
+// contraction), columns of kGroupM row tiles.
+struct Walk {
+  int mt, nt, splits, total;
+  __device__ __forceinline__ void at(int t, int& m, int& n, int& s) const {
+    s = t % splits;
+    t /= splits;
+    const int per = kGroupM * nt;
+    const int g = t / per, r = t - g * per;
+    const int gm = min(kGroupM, mt - g * kGroupM);
+    n = r / gm;
+    m = g * kGroupM + r - n * gm;
+  }
+};
+
+template <int OP>
+__global__ void __launch_bounds__(kThreads, 1)
+    gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Args a) {
+  constexpr bool A_MN = OP == kDw, B_MN = OP == kDh || OP == kDw;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(smem);
+  const uint32_t bar_full = sbase + kStages * kStageBytes;
+  const uint32_t bar_empty = bar_full + kStages * 8;
+  const uint32_t bar_tfull = bar_empty + kStages * 8;  // [2] accumulator complete
+  const uint32_t bar_tempty = bar_tfull + 16;          // [2] accumulator read
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kStages * kStageBytes + kBars * 8);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(bar_tfull + 8 * s, 1);
+      mbar_init(bar_tempty + 8 * s, 128);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 2) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+
+  const int n = *a.count;
+  Walk w;
+  int kb_total;
+  if constexpr (OP == kStats || OP == kGrad) {
+    w.mt = (n + kTileM - 1) / kTileM;
+    w.nt = (a.nv + kTileN - 1) / kTileN;
+    kb_total = (a.K + 63) / 64;
+  } else if constexpr (OP == kDh) {
+    w.mt = (n + kTileM - 1) / kTileM;
+    w.nt = (a.K + kTileN - 1) / kTileN;
+    kb_total = (a.nv + 63) / 64;
+  } else {
+    w.mt = (a.nv + kTileM - 1) / kTileM;
+    w.nt = (a.K + kTileN - 1) / kTileN;
+    kb_total = (n + 63) / 64;
+  }
+  w.splits = OP == kDh ? a.splits : 1;
+  w.total = w.mt * w.nt * w.splits;
+  const int kb_per = (kb_total + w.splits - 1) / w.splits;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint64_t pol = l2_policy_evict_last();
+      int it = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; ok && t < w.total; t += gridDim.x) {
+        int m, nn, s;
+        w.at(t, m, nn, s);
+        const int m0 = m * kTileM, n0 = nn * kTileN;
+        const int kb0 = s * kb_per, kb1 = min(kb_total, kb0 + kb_per);
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int st = it % kStages, r = it / kStages;
+          if (r > 0 && !mbar_wait(bar_empty + 8 * st, (r - 1) & 1, kErrGemmWait)) {
+            ok = false;
+            break;
+          }
+          const uint32_t sa = sbase + st * kStageBytes, sb = sa + kABytes, bar = bar_full + 8 * st;
+          mbar_arrive_expect_tx(bar, kStageBytes);
+          const int kc = kb * 64;
+          if constexpr (A_MN) {
+#pragma unroll
+            for (int j = 0; j < kTileM / 64; ++j) tma_load_2d(sa + j * 8192, &tmA, bar, m0 + 64 * j, kc, pol);
+          } else {
+            tma_load_2d(sa, &tmA, bar, kc, m0, pol);
+          }
+          if constexpr (B_MN) {
+            const int row = OP == kDh ? a.v0 + kc : kc;
+#pragma unroll
+            for (int j = 0; j < kTileN / 64; ++j) tma_load_2d(sb + j * 8192, &tmB, bar, n0 + 64 * j, row, pol);
+          } else {
+            tma_load_2d(sb, &tmB, bar, kc, a.v0 + n0, pol);
+          }
+        }
+      }
+      // no copy issued here may still be landing when the CTA leaves
+      for (int i = max(0, it - kStages); i < it; ++i)
+        mbar_wait(bar_full + 8 * (i % kStages), (i / kStages) & 1, kErrGemmWait);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = umma_idesc_bf16(kTileM, kTileN, A_MN, B_MN);
+      int it = 0, tile = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; ok && t < w.total; t += gridDim.x, ++tile) {
+        int m, nn, s;
+        w.at(t, m, nn, s);
+        const int kb0 = s * kb_per, kb1 = min(kb_total, kb0 + kb_per);
+        const int buf = tile & 1;
+        if (!mbar_wait(bar_tempty + 8 * buf, ((tile >> 1) & 1) ^ 1, kErrTmemWait)) break;
+        tc_fence_after();
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int st = it % kStages, r = it / kStages;
+          if (!mbar_wait(bar_full + 8 * st, r & 1, kErrGemmWait)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = sbase + st * kStageBytes, sb = sa + kABytes;
+          // 16 deep per instruction: K-major tiles step 32 bytes along their rows, MN-major ones 16
+          // rows of 128 bytes
+          const uint64_t ad = A_MN ? umma_desc_mn_sw128(sa, 8192, 1024) : umma_desc_k_sw128(sa, 1024);
+          const uint64_t bd = B_MN ? umma_desc_mn_sw128(sb, 8192, 1024) : umma_desc_k_sw128(sb, 1024);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tc_mma_f16(tmem + buf * kTileN, ad + (A_MN ? 128 : 2) * k, bd + (B_MN ? 128 : 2) * k, idesc,
+                       (kb > kb0 || k > 0) ? 1u : 0u);
+          tc_commit(bar_empty + 8 * st);
+        }
+        tc_commit(bar_tfull + 8 * buf);
+      }
+    }
+  } else if (warp >= 4) {
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const int r = (warp & 3) * 32 + lane;
+    const float inv_n = 1.f / (float)max(n, 1);
+    int tile = 0;
+    for (int t = blockIdx.x; t < w.total; t += gridDim.x, ++tile) {
+      int m, nn, s;
+      w.at(t, m, nn, s);
+      const int row = m * kTileM + r, n0 = nn * kTileN;
+      const int buf = tile & 1;
+      const bool empty = s * kb_per >= kb_total;  // nothing contracted: the product is zero
+      int target = -1;
+      float shift = 0.f, dl = 0.f, at_target = 0.f;
+      if constexpr (OP == kStats || OP == kGrad) {
+        if (row < n) {
+          target = a.target[row] - (a.v0 + n0);  // its column in this tile, if within 0 .. 255
+          if constexpr (OP == kGrad) {
+            const float l = a.loss[row];
+            shift = (a.zt[row] + l) * kLog2e;
+            dl = a.dloss[a.dloss_stride * a.token[row]] * (a.mean ? inv_n : 1.f);
+            at_target = expm1f(-l);
+          }
+        }
+      }
+      const int cols = min(kTileN, (OP == kStats || OP == kGrad ? a.nv : a.K) - n0);
+      const bool ok = mbar_wait(bar_tfull + 8 * buf, (tile >> 1) & 1, kErrTmemWait);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+      float mx = -INFINITY, sum = 0.f;
+#pragma unroll 1
+      for (int c = 0; c < kTileN; c += 32) {
+        uint32_t v[32];
+        tmem_ld32(tmem + lanes + buf * kTileN + c, v);
+        tc_wait_ld();
+        if constexpr (OP == kStats || OP == kGrad) {
+          if (a.cap > 0.f) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(a.cap * tanhf(__uint_as_float(v[j]) * a.inv_cap));
+          }
+        }
+        if constexpr (OP == kStats) {
+          // columns past the vocabulary and the target's take no part
+          if (c + 32 > cols || (unsigned)(target - c) < 32u) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (c + j >= cols || c + j == target) v[j] = 0xff800000u;
+          }
+          float cm = __uint_as_float(v[0]);
+#pragma unroll
+          for (int j = 1; j < 32; ++j) cm = fmaxf(cm, __uint_as_float(v[j]));
+          const float m2 = fmaxf(mx, cm);
+          if (m2 > -INFINITY) {
+            const float off = m2 * kLog2e;
+            sum = mx > -INFINITY ? sum * ex2(mx * kLog2e - off) : sum;  // 0, or NaN that stays
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              s0 += ex2(fmaf(__uint_as_float(v[j]), kLog2e, -off));
+              s1 += ex2(fmaf(__uint_as_float(v[j + 1]), kLog2e, -off));
+            }
+            sum += s0 + s1;
+            mx = m2;
+          } else {
+            // only -inf or NaN so far: NaN has to reach the sum
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sum += __uint_as_float(v[j]) == -INFINITY ? 0.f : __uint_as_float(v[j]);
+          }
+        } else if constexpr (OP == kGrad) {
+          if (row < a.T) {
+            __nv_bfloat16* g = a.G + (int64_t)row * a.ldg + n0 + c;
+            uint32_t o[16];
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              float p[2];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float z = __uint_as_float(v[j + e]);
+                float x = c + j + e == target ? at_target : ex2(fmaf(z, kLog2e, -shift));
+                if (a.cap > 0.f) {
+                  const float q = z * a.inv_cap;
+                  x *= 1.f - q * q;
+                }
+                p[e] = (row < n && c + j + e < cols) ? x * dl : 0.f;
+              }
+              o[j / 2] = pack_bf16x2(p[0], p[1]);
+            }
+            // ldg is a whole number of tiles: columns past the piece are zeros in the buffer
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              reinterpret_cast<uint4*>(g)[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          }
+        } else if constexpr (OP == kDh) {
+          if (row < n) {
+            float* o = a.acc + ((int64_t)s * a.T + row) * a.K + n0 + c;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (c + j < cols) {
+                const float x = empty ? 0.f : __uint_as_float(v[j]);
+                o[j] = a.first ? x : o[j] + x;
+              }
+          }
+        } else {
+          if (row < a.nv) {
+            __nv_bfloat16* o = a.dw + (int64_t)(a.v0 + row) * a.lddw + n0 + c;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (c + j < cols) o[j] = f2bf(empty ? 0.f : __uint_as_float(v[j]));
+          }
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(bar_tempty + 8 * buf);
+      if constexpr (OP == kStats) {
+        if (row < n) a.part[(int64_t)nn * a.T + row] = make_float2(mx, sum);
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 2) tmem_dealloc(tmem, 512);
+}
+
+// ---------------------------------------------------------------------------
+// Gather of the scored rows. A CTA owns `rows` consecutive rows of the batch: it
+// counts the scored ones before them (every CTA reads the targets itself: no
+// second pass, no waiting), then a warp copies a row and takes its target logit.
+// ---------------------------------------------------------------------------
+struct PrepArgs {
+  const __nv_bfloat16* h;
+  const __nv_bfloat16* w;
+  const int64_t* targets;
+  int64_t ldh, ldw;
+  int64_t ignore;
+  __nv_bfloat16* hc;  // [T][Kp] scored rows; Kp a multiple of 8, zero past K
+  int *count, *target, *token, *place;  // place: [T] row of hc, or -1
+  float *zt, *loss;                     // loss: [T] by token (ignored rows: 0)
+  unsigned* ticket;
+  int T, V, K, Kp, rows;
+  float cap, inv_cap;
+};
+
+__global__ void __launch_bounds__(256) prep_kernel(PrepArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  extern __shared__ int dest[];  // [rows]
+  __shared__ int warp_n[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row0 = blockIdx.x * a.rows, row1 = min(a.T, row0 + a.rows);
+  int before = 0;
+  for (int t = threadIdx.x; t < row0; t += 256) before += a.targets[t] != a.ignore;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  if (lane == 0) warp_n[warp] = before;
+  __syncthreads();
+  int base = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) base += warp_n[i];
+  if (warp == 0) {
+    for (int t = row0; t < row1; t += 32) {
+      const bool scored = t + lane < row1 && a.targets[t + lane] != a.ignore;
+      const unsigned b = __ballot_sync(0xffffffffu, scored);
+      if (t + lane < row1) dest[t + lane - row0] = scored ? base + __popc(b & ((1u << lane) - 1)) : -1;
+      base += __popc(b);
+    }
+    if (row1 == a.T) {
+      if (lane == 0) {
+        *a.count = base;
+        *a.ticket = 0;
+        dest[a.rows] = base;
+      }
+    }
+  }
+  __syncthreads();
+  for (int t = row0 + warp; t < row1; t += 8) {
+    const int d = dest[t - row0];
+    if (lane == 0) a.place[t] = d;
+    if (d < 0) {
+      if (lane == 0) a.loss[t] = 0.f;
+      continue;
+    }
+    const int64_t y = a.targets[t];
+    const bool valid = y >= 0 && y < a.V;
+    const __nv_bfloat16* hr = a.h + (int64_t)t * a.ldh;
+    const __nv_bfloat16* wr = a.w + (valid ? y : 0) * a.ldw;
+    __nv_bfloat16* o = a.hc + (int64_t)d * a.Kp;
+    float s = 0.f;
+    for (int c = lane; c < a.Kp; c += 32) {
+      const __nv_bfloat16 x = c < a.K ? hr[c] : f2bf(0.f);
+      o[c] = x;
+      if (c < a.K) s = fmaf(bf2f(x), bf2f(wr[c]), s);
+    }
+    s = warp_sum(s);
+    if (lane == 0) {
+      if (a.cap > 0.f) s = a.cap * tanhf(s * a.inv_cap);
+      if (!valid) {
+        set_status(kErrBounds);
+        s = NAN;
+      }
+      a.zt[d] = s;
+      a.target[d] = valid ? (int)y : -1;
+      a.token[d] = t;
+    }
+  }
+  // rows up to the contraction's next block of 64 take part in dW: zeros
+  if (row1 == a.T) {
+    const int n = dest[a.rows];
+    const int end = min(a.T, (n + 63) / 64 * 64);
+    for (int64_t i = (int64_t)n * a.Kp + threadIdx.x; i < (int64_t)end * a.Kp; i += 256) a.hc[i] = f2bf(0.f);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Merge of the (max, sum) pairs: 32 rows a CTA (lanes), the column tiles dealt to
+// its warps; then each row's loss. The last CTA adds the rows' losses in order.
+// ---------------------------------------------------------------------------
+struct MergeArgs {
+  const float2* part;  // [nt][T]
+  const int *count, *token;
+  const float* zt;
+  float* row_loss;  // [T] by scored row
+  float* loss;      // [T] by token
+  float* total;     // [1] sum or mean, or null
+  unsigned* ticket;
+  int T, nt, mean;
+};
+constexpr int kMergeWarps = 16;
+
+__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
+  const float top = fmaxf(m, m2);
+  if (top > -INFINITY) {
+    s = s * (m > -INFINITY ? ex2((m - top) * kLog2e) : 1.f) + s2 * (m2 > -INFINITY ? ex2((m2 - top) * kLog2e) : 1.f);
+    m = top;
+  } else {
+    s += s2;
+  }
+}
+
+__global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(MergeArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  __shared__ float2 sh[kMergeWarps][32];
+  __shared__ float red[32];
+  __shared__ bool last;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int n = *a.count;
+  const int row = blockIdx.x * 32 + lane;
+  float m = -INFINITY, s = 0.f;
+  if (row < n)
+    for (int t = warp; t < a.nt; t += kMergeWarps) {
+      const float2 p = a.part[(int64_t)t * a.T + row];
+      join(m, s, p.x, p.y);
+    }
+  sh[warp][lane] = make_float2(m, s);
+  __syncthreads();
+  if (warp == 0 && row < n) {
+    for (int i = 1; i < kMergeWarps; ++i) join(m, s, sh[i][lane].x, sh[i][lane].y);
+    // s = 0 (a vocabulary of one): d = -inf, loss 0
+    const float d = m + logf(s) - a.zt[row];
+    const float l = d == -INFINITY ? 0.f : fmaxf(d, 0.f) + log1pf(expf(-fabsf(d)));
+    const float loss = d != d ? d : l;
+    a.row_loss[row] = loss;
+    a.loss[a.token[row]] = loss;
+  }
+  if (a.total == nullptr) return;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  float acc = 0.f;
+  for (int i = threadIdx.x; i < n; i += 32 * kMergeWarps) acc += __ldcg(a.row_loss + i);
+  acc = block_sum(acc, red);
+  if (threadIdx.x == 0) *a.total = a.mean ? acc / (float)max(n, 1) : acc;
+}
+
+// dh[t] = sum over the contraction's parts of acc[.][place[t]], 0 for ignored rows.
+__global__ void __launch_bounds__(256) finish_dh_kernel(const float* acc, const int* place, __nv_bfloat16* dh, int T,
+                                                        int K, int splits) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t total = (int64_t)T * K;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int t = (int)(i / K);
+    const int c = (int)(i - (int64_t)t * K);
+    const int p = place[t];
+    float s = 0.f;
+    if (p >= 0)
+      for (int k = 0; k < splits; ++k) s += acc[((int64_t)k * T + p) * K + c];
+    dh[i] = f2bf(s);
+  }
+}
+
+template <int OP>
+static int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const Args& a, int64_t tiles, int num_sms,
+                       cudaStream_t st) {
+  if (tiles <= 0) return 0;
+  if (tiles > 0x7FFFFFFFll - 1024) return -1;
+  if (int e = smem_attr_once<gemm_kernel<OP>>(kSmem)) return e;
+  const int grid = (int)(tiles < num_sms ? tiles : num_sms);
+  cudaError_t e = launch_k(gemm_kernel<OP>, dim3(grid), dim3(kThreads), kSmem, st, 1, ta, tb, a);
+  return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
+}
+
+static inline int64_t tiles_of(int64_t n, int tile) { return (n + tile - 1) / tile; }
+
+}  // namespace lce
+}  // namespace b200
+
+using namespace b200;
+using namespace b200::lce;
+
+extern "C" {
+
+// Workspace shapes. Column tiles of the statistics: ceil(V / 256).
+int b200_lce_tile_cols() { return kTileN; }
+
+// Parts of the contraction of dh for T rows of K columns: enough tiles for every
+// SM where the rows alone give too few (a part keeps 16 blocks of 64 or more).
+int b200_lce_dh_splits(int T, int K, int piece, int num_sms) {
+  const int64_t tiles = tiles_of(T, kTileM) * tiles_of(K, kTileN);
+  int64_t s = tiles ? num_sms / tiles : 1;
+  const int64_t most = piece / 64 / 16;
+  s = s > most ? most : s;
+  return (int)(s > 64 ? 64 : s < 1 ? 1 : s);
+}
+
+// Forward. h [T, K] and W [V, K] bf16 (strides in elements; W 16-byte aligned with
+// ldw % 8 == 0), targets int64. hc [T, Kp], ints [3 T + 2] (count, ticket, target,
+// token, place), floats [2 T] (zt, row loss), part fp32 [2 ceil(V / 256) T]; loss
+// [T]; total [1] or null (mean: divided by the scored rows, at least 1).
+// Returns 0, a CUDA error code, or -1 for arguments out of range.
+int b200_lce_forward(const void* h, int64_t ldh, const void* W, int64_t ldw, const int64_t* targets, int64_t ignore,
+                     int T, int V, int K, int Kp, float cap, void* hc, int* ints, float* floats, float* part,
+                     float* loss, float* total, int mean, int num_sms, cudaStream_t st) {
+  if (T <= 0 || V <= 0 || K <= 0 || Kp < K || (Kp % 8) || (ldw % 8) || ((uintptr_t)W & 15) || ((uintptr_t)hc & 15))
+    return -1;
+  PrepArgs p = {};
+  p.h = reinterpret_cast<const __nv_bfloat16*>(h);
+  p.w = reinterpret_cast<const __nv_bfloat16*>(W);
+  p.targets = targets;
+  p.ldh = ldh;
+  p.ldw = ldw;
+  p.ignore = ignore;
+  p.hc = reinterpret_cast<__nv_bfloat16*>(hc);
+  p.count = ints;
+  p.ticket = reinterpret_cast<unsigned*>(ints + 1);
+  p.target = ints + 2;
+  p.token = ints + 2 + (int64_t)T;
+  p.place = ints + 2 + 2 * (int64_t)T;
+  p.zt = floats;
+  p.loss = loss;
+  p.T = T;
+  p.V = V;
+  p.K = K;
+  p.Kp = Kp;
+  p.cap = cap;
+  p.inv_cap = cap > 0.f ? 1.f / cap : 0.f;
+  // eight rows a CTA (one a warp) while that is at most four CTAs an SM
+  const int64_t want = tiles_of(T, 4 * num_sms);
+  p.rows = (int)(want < 8 ? 8 : want > 8192 ? 8192 : (want + 7) / 8 * 8);
+  cudaError_t e = launch_k(prep_kernel, dim3((unsigned)tiles_of(T, p.rows)), dim3(256), (p.rows + 1) * sizeof(int), st, 1, p);
+  if (e != cudaSuccess) return (int)e;
+  Args a = {};
+  a.count = p.count;
+  a.target = p.target;
+  a.token = p.token;
+  a.zt = p.zt;
+  a.part = reinterpret_cast<float2*>(part);
+  a.T = T;
+  a.V = V;
+  a.K = K;
+  a.nv = V;
+  a.cap = p.cap;
+  a.inv_cap = p.inv_cap;
+  CUtensorMap ta, tb;
+  if (!make_tmap_2d(&ta, hc, T, Kp, Kp, kTileM, 64, 2) || !make_tmap_2d(&tb, W, V, K, ldw, kTileN, 64, 2)) return -1;
+  if (int r = launch_gemm<kStats>(ta, tb, a, tiles_of(T, kTileM) * tiles_of(V, kTileN), num_sms, st)) return r;
+  MergeArgs g = {};
+  g.part = a.part;
+  g.count = p.count;
+  g.token = p.token;
+  g.zt = p.zt;
+  g.row_loss = floats + T;
+  g.loss = loss;
+  g.total = total;
+  g.ticket = p.ticket;
+  g.T = T;
+  g.nt = (int)tiles_of(V, kTileN);
+  g.mean = mean;
+  e = launch_k(merge_kernel, dim3((unsigned)tiles_of(T, 32)), dim3(32 * kMergeWarps), 0, st, 1, g);
+  return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
+}
+
+// Backward from the forward's hc, ints and floats. dloss: element token *
+// dloss_stride. dh [T, K] contiguous and dW [V, K] (row stride lddw) are null where
+// not wanted. piece: columns of the vocabulary at a time, a multiple of 256; G bf16
+// [T, piece]; acc fp32 [splits, T, K] for dh.
+int b200_lce_backward(const void* hc, const void* W, int64_t ldw, const int* ints, const float* floats,
+                      const float* dloss, int64_t dloss_stride, int mean, int T, int V, int K, int Kp, float cap,
+                      int piece, void* G, float* acc, int splits, void* dh, void* dW, int64_t lddw, int num_sms,
+                      cudaStream_t st) {
+  if (T <= 0 || V <= 0 || K <= 0 || Kp < K || (Kp % 8) || (ldw % 8) || ((uintptr_t)W & 15) || piece <= 0 ||
+      (piece % kTileN) || splits < 1 || ((uintptr_t)G & 15) || (dh && !acc))
+    return -1;
+  Args a = {};
+  a.count = ints;
+  a.target = ints + 2;
+  a.token = ints + 2 + (int64_t)T;
+  const int* place = ints + 2 + 2 * (int64_t)T;
+  a.zt = floats;
+  a.loss = floats + T;
+  a.dloss = dloss;
+  a.dloss_stride = dloss_stride;
+  a.mean = mean;
+  a.G = reinterpret_cast<__nv_bfloat16*>(G);
+  a.ldg = piece;
+  a.acc = acc;
+  a.dw = reinterpret_cast<__nv_bfloat16*>(dW);
+  a.lddw = lddw;
+  a.T = T;
+  a.V = V;
+  a.K = K;
+  a.splits = splits;
+  a.cap = cap;
+  a.inv_cap = cap > 0.f ? 1.f / cap : 0.f;
+  CUtensorMap h_rows, w_rows, g_rows, w_cols, g_cols, h_cols;
+  if (!make_tmap_2d(&h_rows, hc, T, Kp, Kp, kTileM, 64, 2) || !make_tmap_2d(&w_rows, W, V, K, ldw, kTileN, 64, 2) ||
+      !make_tmap_2d(&g_rows, G, T, piece, piece, kTileM, 64, 2) || !make_tmap_2d(&w_cols, W, V, K, ldw, 64, 64, 2) ||
+      !make_tmap_2d(&g_cols, G, T, piece, piece, 64, 64, 2) || !make_tmap_2d(&h_cols, hc, T, Kp, Kp, 64, 64, 2))
+    return -1;
+  for (int64_t v0 = 0; v0 < V; v0 += piece) {
+    a.v0 = (int)v0;
+    a.nv = (int)(V - v0 < piece ? V - v0 : piece);
+    a.first = v0 == 0;
+    if (int r = launch_gemm<kGrad>(h_rows, w_rows, a, tiles_of(T, kTileM) * tiles_of(a.nv, kTileN), num_sms, st)) return r;
+    if (dh)
+      if (int r = launch_gemm<kDh>(g_rows, w_cols, a, tiles_of(T, kTileM) * tiles_of(K, kTileN) * splits, num_sms, st)) return r;
+    if (dW)
+      if (int r = launch_gemm<kDw>(g_cols, h_cols, a, tiles_of(a.nv, kTileM) * tiles_of(K, kTileN), num_sms, st)) return r;
+  }
+  if (dh) {
+    const int64_t blocks = tiles_of((int64_t)T * K, 256);
+    cudaError_t e = launch_k(finish_dh_kernel, dim3((unsigned)(blocks < 8 * num_sms ? blocks : 8 * num_sms)), dim3(256), 0,
+                             st, 1, acc, place, reinterpret_cast<__nv_bfloat16*>(dh), T, K, splits);
+    if (e != cudaSuccess) return (int)e;
+  }
+  return (int)cudaGetLastError();
+}
+
+}  // extern "C"
+
+B200_STATUS_ACCESSORS(linear_ce)

@@ -7,10 +7,11 @@ Parity: LoRALinear's dropout before the A product (LoRA+Layers.swift:109).
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from . import reference as ref
-from ._args import elem_code, rows2d, same_device
+from ._args import ELEM, elem_code, rows2d, same_device
 from .linear import num_sms
 
 _lib.register_signatures({
@@ -21,19 +22,17 @@ _lib.register_signatures({
 
 def _launch(x, p, seed, offset, residual):
     cut = ref.dropout_cut(p)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     if x.numel() == 0:
         return y
     K = x.shape[-1] if x.dim() else 1
     x2 = rows2d(x, K)
     r2 = None if residual is None else rows2d(residual, K)
-    dev_offset = isinstance(offset, torch.Tensor)
-    with torch.cuda.device(x.device):
-        rc = _lib.lib().b200_dropout(
-            x2.data_ptr(), x2.stride(0), _lib.ptr(r2), 0 if r2 is None else r2.stride(0), y.data_ptr(), K,
-            x2.shape[0], K, elem_code(x, "dropout"), seed, 0 if dev_offset else offset,
-            offset.data_ptr() if dev_offset else None, cut, ref.dropout_scale(cut), num_sms(x.device),
-            _lib.stream_ptr(x.device))
+    host_offset, dev_offset = (0, offset.data_ptr()) if isinstance(offset, torch.Tensor) else (offset, None)
+    rc = _lib.launch(_lib.lib().b200_dropout, x.device, x2.data_ptr(), x2.stride(0),
+                     None if r2 is None else r2.data_ptr(), 0 if r2 is None else r2.stride(0), y.data_ptr(), K,
+                     x2.shape[0], K, ELEM[x.dtype], seed, host_offset, dev_offset, cut, ref.dropout_scale(cut),
+                     num_sms(x.device))
     _lib.check(rc, "dropout")
     _lib.count(1)
     return y
@@ -48,6 +47,7 @@ class _Dropout(torch.autograd.Function):
         return _launch(x, p, seed, ctx.offset, residual)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         dx = _launch(dy, ctx.p, ctx.seed, ctx.offset, None) if ctx.needs_input_grad[0] else None
         return dx, dy if ctx.needs_input_grad[1] else None, None, None, None

@@ -2,10 +2,11 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from . import reference as ref
-from ._args import elem_code, rows2d, same_device
+from ._args import ELEM, elem_code, rows2d, same_device
 from .linear import num_sms
 
 _lib.register_signatures({
@@ -93,8 +94,8 @@ def _block_norms_fwd(x, delta, post_w, pre_w, gate, kind, eps, scale, offset_one
     H = x.shape[-1]
     dev = x.device
     if y is None:
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    h = None if pre_w is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    h = None if pre_w is None else torch.empty_like(x, memory_format=torch.contiguous_format)
     x2, d2, y2 = rows2d(x, H), rows2d(delta, H), rows2d(y, H)
     T = x2.shape[0]
     r1 = torch.empty(T, dtype=torch.float32, device=dev) if save and post_w is not None else None
@@ -103,13 +104,12 @@ def _block_norms_fwd(x, delta, post_w, pre_w, gate, kind, eps, scale, offset_one
     g = None if gate is None else rows2d(gate, H) if kind == _GATE_ELEMENT else gate.contiguous()
     w = post_w if post_w is not None else pre_w
     if T:
-        with torch.cuda.device(dev):
-            rc = _lib.lib().b200_block_norms(
-                x2.data_ptr(), x2.stride(0), d2.data_ptr(), d2.stride(0), _lib.ptr(post_w), _lib.ptr(pre_w),
-                0 if w is None else elem_code(w, "block_norms weight"), _lib.ptr(g),
-                g.stride(0) if kind == _GATE_ELEMENT else 0, kind, y2.data_ptr(), y2.stride(0), _lib.ptr(h), H,
-                _lib.ptr(r1), _lib.ptr(r2), T, H, elem_code(x, "block_norms"), float(eps), float(scale),
-                1 if offset_one else 0, 1 if round_branch else 0, _lib.stream_ptr(dev))
+        rc = _lib.launch(
+            _lib.lib().b200_block_norms, dev, x2.data_ptr(), x2.stride(0), d2.data_ptr(), d2.stride(0),
+            _lib.ptr(post_w), _lib.ptr(pre_w), 0 if w is None else ELEM[w.dtype], _lib.ptr(g),
+            g.stride(0) if kind == _GATE_ELEMENT else 0, kind, y2.data_ptr(), y2.stride(0), _lib.ptr(h), H,
+            _lib.ptr(r1), _lib.ptr(r2), T, H, ELEM[x.dtype], float(eps), float(scale), 1 if offset_one else 0,
+            1 if round_branch else 0)
         _lib.check(rc, "block_norms")
         _lib.count(1)
     return y, h, r1, r2
@@ -126,6 +126,7 @@ class _BlockNorms(torch.autograd.Function):
         return y, h
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, dh=None):
         y, delta, post_w, pre_w, gate, r1, r2 = ctx.saved_tensors
         need_x, need_d, need_post, need_pre, need_gate = ctx.needs_input_grad[:5]
@@ -135,7 +136,7 @@ class _BlockNorms(torch.autograd.Function):
         dev, H, kind = y.device, y.shape[-1], ctx.kind
 
         def like(t, need):
-            return torch.empty(t.shape, dtype=t.dtype, device=dev) if need else None
+            return torch.empty_like(t, memory_format=torch.contiguous_format) if need else None
 
         y2, d2 = rows2d(y, H), rows2d(delta, H)
         T = y2.shape[0]
@@ -155,14 +156,12 @@ class _BlockNorms(torch.autograd.Function):
         L, sms = _lib.lib(), num_sms(dev)
         part = (torch.empty(n_part * L.b200_block_norms_bwd_grid(T, H, sms) * H, dtype=torch.float32, device=dev)
                 if n_part else None)
-        with torch.cuda.device(dev):
-            rc = L.b200_block_norms_bwd(
-                y2.data_ptr(), y2.stride(0), d2.data_ptr(), d2.stride(0), _lib.ptr(pw), _lib.ptr(qw),
-                0 if w is None else elem_code(w, "block_norms weight"), _lib.ptr(g),
-                g.stride(0) if kind == _GATE_ELEMENT else 0, kind, _lib.ptr(r1), _lib.ptr(r2), _lib.ptr(dy2),
-                0 if dy2 is None else dy2.stride(0), _lib.ptr(dh2), 0 if dh2 is None else dh2.stride(0),
-                _lib.ptr(dx), _lib.ptr(dd), _lib.ptr(dgate), _lib.ptr(dpost), _lib.ptr(dpre), _lib.ptr(part), T, H,
-                elem_code(y, "block_norms"), ctx.scale, 1 if ctx.offset_one else 0, sms, _lib.stream_ptr(dev))
+        rc = _lib.launch(
+            L.b200_block_norms_bwd, dev, y2.data_ptr(), y2.stride(0), d2.data_ptr(), d2.stride(0), _lib.ptr(pw),
+            _lib.ptr(qw), 0 if w is None else ELEM[w.dtype], _lib.ptr(g), g.stride(0) if kind == _GATE_ELEMENT else 0,
+            kind, _lib.ptr(r1), _lib.ptr(r2), _lib.ptr(dy2), 0 if dy2 is None else dy2.stride(0), _lib.ptr(dh2),
+            0 if dh2 is None else dh2.stride(0), _lib.ptr(dx), _lib.ptr(dd), _lib.ptr(dgate), _lib.ptr(dpost),
+            _lib.ptr(dpre), _lib.ptr(part), T, H, ELEM[y.dtype], ctx.scale, 1 if ctx.offset_one else 0, sms)
         _lib.check(rc, "block_norms backward")
         _lib.count(2 if n_part else 1)
         return (dx, dd, dpost, dpre, dgate) + none

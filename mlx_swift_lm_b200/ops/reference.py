@@ -566,3 +566,21 @@ def block_norms_ref(x, delta, post_w, pre_w, eps, gate=None, scale=1.0, offset_o
         u = u * gate.float()
     y = (x.float() + scale * u).to(x.dtype)
     return y, None if pre_w is None else rms(y.float(), pre_w).to(x.dtype)
+
+
+def linear_cross_entropy_ref(h, w, targets, softcap=0.0, ignore_index=-100, reduction="none"):
+    """:func:`ops.linear_cross_entropy` with the logits in memory; differentiable.
+    Only scored rows enter, so nothing an ignored row holds reaches a gradient."""
+    t = targets.reshape(-1)
+    scored = t != ignore_index
+    z = h.reshape(-1, h.shape[-1])[scored].float() @ w.float().t()
+    if softcap > 0:
+        z = softcap * torch.tanh(z / softcap)
+    y = t[scored]
+    zt = z.gather(1, y[:, None])[:, 0]
+    d = torch.logsumexp(z.scatter(1, y[:, None], -math.inf), 1) - zt
+    each = torch.nn.functional.softplus(d, threshold=1e9)
+    loss = torch.zeros(t.shape[0], dtype=torch.float32, device=h.device).masked_scatter(scored, each)
+    if reduction == "none":
+        return loss.reshape(targets.shape)
+    return loss.sum() if reduction == "sum" else loss.sum() / scored.sum().clamp_min(1)
