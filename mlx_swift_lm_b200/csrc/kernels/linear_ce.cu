@@ -20,11 +20,14 @@
 // count stays on the device, so padding costs nothing and whatever ignored rows
 // hold (NaN included) reaches no gradient.
 //
-// One kernel does the four products (Op): persistent CTAs, one per SM, walk 128 x
-// 256 output tiles. Warp 0 fetches operands by TMA into a ring of 64-deep stages,
-// warp 1 issues tcgen05.mma into one of two accumulators in tensor memory (2 x
-// 256 columns), warps 4 - 7 work on the other one's finished tile, a row of it
-// per thread: the softmax arithmetic runs under the next tile's product.
+// One kernel does the four products (Op): persistent pairs of CTAs on neighbouring
+// SMs walk 256 x 256 output tiles (tcgen05.mma.cta_group::2: each CTA holds half of
+// either operand's rows and half of the accumulator's). Per CTA, warp 0 fetches its
+// operand halves by TMA into a ring of 64-deep stages, one thread of the pair issues
+// the MMAs into one of two accumulators in tensor memory (2 x 256 columns), and warps
+// 4 - 7 work on the other one's finished tile, a row of it per thread: the softmax
+// arithmetic and the stores run under the next tile's product. Tiles leave through
+// shared memory by TMA; the fp32 sums of dh are added up in L2 by its reduction.
 #include "b200_common.cuh"
 
 namespace b200 {
@@ -53,23 +56,92 @@ struct Args {
   int64_t dloss_stride;
   int mean;              // dloss is of the mean: divide by n
   float2* part;          // kStats: [tiles of 256 columns][T]
-  __nv_bfloat16* G;      // [T][ldg]
-  int64_t ldg;
-  float* acc;            // kDh: [splits][T][K]
-  __nv_bfloat16* dw;     // kDw: [V][K]
-  int64_t lddw;
+  int acc_rows;          // kDh: rows of one part of the fp32 sums (whole half tiles, so that none reaches into the next)
   int T, V, K;
   int v0, nv;            // the piece's first column and columns
   int splits, first;     // kDh: parts of the contraction; first piece stores, others add
   float cap, inv_cap;    // cap 0: none
 };
 
-constexpr int kTileM = 128, kTileN = 256, kStages = 4;
-constexpr int kABytes = kTileM * 128, kBBytes = kTileN * 128, kStageBytes = kABytes + kBBytes;
+constexpr int kTileM = 256, kTileN = 256, kStages = 6;  // of a pair of CTAs
+constexpr int kRowsM = kTileM / 2, kRowsN = kTileN / 2;   // a CTA's share of either operand
+constexpr int kABytes = kRowsM * 128, kBBytes = kRowsN * 128, kStageBytes = kABytes + kBBytes;
+constexpr int kOutBytes = kRowsM * 128;  // one of two staging buffers: 128 rows of 128 bytes
 constexpr int kBars = 2 * kStages + 4;
-constexpr int kSmem = kStages * kStageBytes + kBars * 8 + 16 + 1024;
+constexpr int kBarOffset = kStages * kStageBytes + 2 * kOutBytes;
+constexpr int kSmem = kBarOffset + kBars * 8 + 16 + 1024;
 constexpr int kThreads = 256;
-constexpr int kGroupM = 16;  // row tiles walked per column tile before the next: W is read once per 16 x 128 rows, h stays in L2
+constexpr int kEpiWarps = 4;
+constexpr int kGroupM = 16;  // row tiles walked per column tile before the next: W is read once per 16 x 256 rows, h stays in L2
+static_assert(kSmem <= 227 * 1024, "shared memory plan exceeds the per-CTA limit");
+
+// --- tcgen05 on a pair of CTAs ---
+__device__ __forceinline__ void tmem_alloc2(uint32_t dst_smem, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(ncols) : "memory");
+}
+__device__ __forceinline__ void tmem_relinquish2() {
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc2(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+__device__ __forceinline__ void mma2_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrive on the barrier at this shared-memory offset in both CTAs once all MMAs issued so far are complete.
+__device__ __forceinline__ void commit2(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"((uint16_t)3)
+      : "memory");
+}
+// Address of a shared-memory variable of the pair's first CTA.
+__device__ __forceinline__ uint32_t in_leader(uint32_t addr) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+// Load into this CTA's shared memory, counted on a barrier of the pair's first CTA.
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* m, uint32_t cluster_bar, int c0, int c1,
+                                              uint64_t hint) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%2, %3}], [%4], %5;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(c0), "r"(c1), "r"(cluster_bar), "l"(hint)
+      : "memory");
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// --- tiles to global memory ---
+__device__ __forceinline__ void tma_store(const CUtensorMap* m, uint32_t src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(m)),
+               "r"(src), "r"(c0), "r"(c1)
+               : "memory");
+}
+__device__ __forceinline__ void tma_add_f32(const CUtensorMap* m, uint32_t src, int c0, int c1) {
+  asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(m)),
+               "r"(src), "r"(c0), "r"(c1)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void epi_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory"); }
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -92,19 +164,28 @@ struct Walk {
   }
 };
 
+// Gradient of the loss with respect to the target's logit before the cap.
+__device__ __forceinline__ float target_grad(const Args& a, int row, float inv_n) {
+  const float q = a.zt[row] * a.inv_cap;  // inv_cap 0: no cap
+  return expm1f(-a.loss[row]) * (1.f - q * q) * a.dloss[a.dloss_stride * a.token[row]] * (a.mean ? inv_n : 1.f);
+}
+
 template <int OP>
-__global__ void __launch_bounds__(kThreads, 1)
-    gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Args a) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                const __grid_constant__ CUtensorMap tmO, const Args a) {
   constexpr bool A_MN = OP == kDw, B_MN = OP == kDh || OP == kDw;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
-  const uint32_t bar_full = sbase + kStages * kStageBytes;
-  const uint32_t bar_empty = bar_full + kStages * 8;
-  const uint32_t bar_tfull = bar_empty + kStages * 8;  // [2] accumulator complete
-  const uint32_t bar_tempty = bar_tfull + 16;          // [2] accumulator read
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kStages * kStageBytes + kBars * 8);
+  const uint32_t out_smem = sbase + kStages * kStageBytes;
+  const uint32_t bar_full = sbase + kBarOffset;        // the first CTA's: both CTAs' operands in place
+  const uint32_t bar_empty = bar_full + kStages * 8;   // each CTA's: stage consumed
+  const uint32_t bar_tfull = bar_empty + kStages * 8;  // [2] each CTA's: accumulator complete
+  const uint32_t bar_tempty = bar_tfull + 16;          // [2] the first CTA's: accumulator read by both
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kBarOffset + kBars * 8);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
@@ -116,16 +197,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(bar_tfull + 8 * s, 1);
-      mbar_init(bar_tempty + 8 * s, 128);
+      mbar_init(bar_tempty + 8 * s, 2 * kEpiWarps);
     }
     fence_barrier_init();
   }
   if (warp == 2) {
-    tmem_alloc(smem_u32(tmem_slot), 512);
-    tmem_relinquish();
+    tmem_alloc2(smem_u32(tmem_slot), 512);
+    tmem_relinquish2();
   }
   tc_fence_before();
   __syncthreads();
+  cluster_barrier();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
@@ -155,10 +237,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t pol = l2_policy_evict_last();
       int it = 0;
       bool ok = true;
-      for (int t = blockIdx.x; ok && t < w.total; t += gridDim.x) {
+      for (int t = pair; ok && t < w.total; t += pairs) {
         int m, nn, s;
         w.at(t, m, nn, s);
-        const int m0 = m * kTileM, n0 = nn * kTileN;
+        const int m0 = m * kTileM + rank * kRowsM, n0 = nn * kTileN + rank * kRowsN;
         const int kb0 = s * kb_per, kb1 = min(kb_total, kb0 + kb_per);
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int st = it % kStages, r = it / kStages;
@@ -166,34 +248,36 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = false;
             break;
           }
-          const uint32_t sa = sbase + st * kStageBytes, sb = sa + kABytes, bar = bar_full + 8 * st;
-          mbar_arrive_expect_tx(bar, kStageBytes);
+          const uint32_t sa = sbase + st * kStageBytes, sb = sa + kABytes;
+          const uint32_t bar = in_leader(bar_full + 8 * st);
+          if (rank == 0) mbar_arrive_expect_tx(bar_full + 8 * st, 2 * kStageBytes);
           const int kc = kb * 64;
           if constexpr (A_MN) {
 #pragma unroll
-            for (int j = 0; j < kTileM / 64; ++j) tma_load_2d(sa + j * 8192, &tmA, bar, m0 + 64 * j, kc, pol);
+            for (int j = 0; j < kRowsM / 64; ++j) tma_load_pair(sa + j * 8192, &tmA, bar, m0 + 64 * j, kc, pol);
           } else {
-            tma_load_2d(sa, &tmA, bar, kc, m0, pol);
+            tma_load_pair(sa, &tmA, bar, kc, m0, pol);
           }
           if constexpr (B_MN) {
             const int row = OP == kDh ? a.v0 + kc : kc;
 #pragma unroll
-            for (int j = 0; j < kTileN / 64; ++j) tma_load_2d(sb + j * 8192, &tmB, bar, n0 + 64 * j, row, pol);
+            for (int j = 0; j < kRowsN / 64; ++j) tma_load_pair(sb + j * 8192, &tmB, bar, n0 + 64 * j, row, pol);
           } else {
-            tma_load_2d(sb, &tmB, bar, kc, a.v0 + n0, pol);
+            tma_load_pair(sb, &tmB, bar, kc, a.v0 + n0, pol);
           }
         }
       }
-      // no copy issued here may still be landing when the CTA leaves
+      // every stage filled here has been consumed before the CTA leaves, so that no copy
+      // and no arrival on its barriers is still under way
       for (int i = max(0, it - kStages); i < it; ++i)
-        mbar_wait(bar_full + 8 * (i % kStages), (i / kStages) & 1, kErrGemmWait);
+        mbar_wait(bar_empty + 8 * (i % kStages), (i / kStages) & 1, kErrGemmWait);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       constexpr uint32_t idesc = umma_idesc_bf16(kTileM, kTileN, A_MN, B_MN);
       int it = 0, tile = 0;
       bool ok = true;
-      for (int t = blockIdx.x; ok && t < w.total; t += gridDim.x, ++tile) {
+      for (int t = pair; ok && t < w.total; t += pairs, ++tile) {
         int m, nn, s;
         w.at(t, m, nn, s);
         const int kb0 = s * kb_per, kb1 = min(kb_total, kb0 + kb_per);
@@ -214,54 +298,53 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint64_t bd = B_MN ? umma_desc_mn_sw128(sb, 8192, 1024) : umma_desc_k_sw128(sb, 1024);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            tc_mma_f16(tmem + buf * kTileN, ad + (A_MN ? 128 : 2) * k, bd + (B_MN ? 128 : 2) * k, idesc,
-                       (kb > kb0 || k > 0) ? 1u : 0u);
-          tc_commit(bar_empty + 8 * st);
+            mma2_f16(tmem + buf * kTileN, ad + (A_MN ? 128 : 2) * k, bd + (B_MN ? 128 : 2) * k, idesc,
+                     (kb > kb0 || k > 0) ? 1u : 0u);
+          commit2(bar_empty + 8 * st);
         }
-        tc_commit(bar_tfull + 8 * buf);
+        commit2(bar_tfull + 8 * buf);
       }
     }
   } else if (warp >= 4) {
+    const int r = (warp & 3) * 32 + lane;  // row of the CTA's half tile = tensor-memory lane
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const int r = (warp & 3) * 32 + lane;
     const float inv_n = 1.f / (float)max(n, 1);
-    int tile = 0;
-    for (int t = blockIdx.x; t < w.total; t += gridDim.x, ++tile) {
+    const uint32_t release = in_leader(bar_tempty);
+    int tile = 0, out = 0;
+    for (int t = pair; t < w.total; t += pairs, ++tile) {
       int m, nn, s;
       w.at(t, m, nn, s);
-      const int row = m * kTileM + r, n0 = nn * kTileN;
+      const int m0 = m * kTileM + rank * kRowsM, row = m0 + r, n0 = nn * kTileN;
       const int buf = tile & 1;
+      const uint32_t acc = tmem + lanes + buf * kTileN;
       const bool empty = s * kb_per >= kb_total;  // nothing contracted: the product is zero
+      const int cols = min(kTileN, (OP == kStats || OP == kGrad ? a.nv : a.K) - n0);
       int target = -1;
       float shift = 0.f, dl = 0.f, at_target = 0.f;
       if constexpr (OP == kStats || OP == kGrad) {
         if (row < n) {
           target = a.target[row] - (a.v0 + n0);  // its column in this tile, if within 0 .. 255
           if constexpr (OP == kGrad) {
-            const float l = a.loss[row];
-            shift = (a.zt[row] + l) * kLog2e;
+            shift = (a.zt[row] + a.loss[row]) * kLog2e;
             dl = a.dloss[a.dloss_stride * a.token[row]] * (a.mean ? inv_n : 1.f);
-            at_target = expm1f(-l);
+            at_target = target_grad(a, row, inv_n);
           }
         }
       }
-      const int cols = min(kTileN, (OP == kStats || OP == kGrad ? a.nv : a.K) - n0);
       const bool ok = mbar_wait(bar_tfull + 8 * buf, (tile >> 1) & 1, kErrTmemWait);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
-      float mx = -INFINITY, sum = 0.f;
+      if constexpr (OP == kStats) {
+        float mx = -INFINITY, sum = 0.f;
 #pragma unroll 1
-      for (int c = 0; c < kTileN; c += 32) {
-        uint32_t v[32];
-        tmem_ld32(tmem + lanes + buf * kTileN + c, v);
-        tc_wait_ld();
-        if constexpr (OP == kStats || OP == kGrad) {
+        for (int c = 0; c < cols; c += 32) {
+          uint32_t v[32];
+          tmem_ld32(acc + c, v);
+          tc_wait_ld();
           if (a.cap > 0.f) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(a.cap * tanhf(__uint_as_float(v[j]) * a.inv_cap));
           }
-        }
-        if constexpr (OP == kStats) {
           // columns past the vocabulary and the target's take no part
           if (c + 32 > cols || (unsigned)(target - c) < 32u) {
 #pragma unroll
@@ -288,61 +371,95 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int j = 0; j < 32; ++j) sum += __uint_as_float(v[j]) == -INFINITY ? 0.f : __uint_as_float(v[j]);
           }
-        } else if constexpr (OP == kGrad) {
-          if (row < a.T) {
-            __nv_bfloat16* g = a.G + (int64_t)row * a.ldg + n0 + c;
-            uint32_t o[16];
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_cluster(release + 8 * buf);
+        if (row < n) a.part[(int64_t)nn * a.T + row] = make_float2(mx, sum);
+      } else {
+        // 128 bytes of a row at a time (64 bf16 or 32 fp32) through one of two staging buffers
+        // in the 128-byte swizzle, stored by one thread while the next ones are filled
+        constexpr int kStep = OP == kDh ? 32 : 64;
+        const bool any_row = OP == kDw ? m0 < a.nv : m0 < n;
+#pragma unroll 1
+        for (int c = 0; c < cols; c += kStep, ++out) {
+          uint32_t o[32];
+          if constexpr (OP == kGrad) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              float p[2];
+            for (int hh = 0; hh < 64; hh += 32) {
+              uint32_t v[32];
+              tmem_ld32(acc + c + hh, v);
+              tc_wait_ld();
+              const int rel = target - (c + hh);
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const float z = __uint_as_float(v[j + e]);
-                float x = c + j + e == target ? at_target : ex2(fmaf(z, kLog2e, -shift));
-                if (a.cap > 0.f) {
-                  const float q = z * a.inv_cap;
-                  x *= 1.f - q * q;
+              for (int j = 0; j < 32; j += 2) {
+                float p[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  float z = __uint_as_float(v[j + e]), slope = dl;
+                  if (a.cap > 0.f) {
+                    const float q = tanhf(z * a.inv_cap);
+                    z = a.cap * q;
+                    slope *= 1.f - q * q;
+                  }
+                  p[e] = ex2(fmaf(z, kLog2e, -shift)) * slope;
+                  if (rel == j + e) p[e] = at_target;
+                  if (row >= n || c + hh + j + e >= cols) p[e] = 0.f;
                 }
-                p[e] = (row < n && c + j + e < cols) ? x * dl : 0.f;
+                o[(hh + j) / 2] = pack_bf16x2(p[0], p[1]);
               }
-              o[j / 2] = pack_bf16x2(p[0], p[1]);
             }
-            // ldg is a whole number of tiles: columns past the piece are zeros in the buffer
+          } else if constexpr (OP == kDh) {
+            tmem_ld32(acc + c, o);
+            tc_wait_ld();
+          } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              reinterpret_cast<uint4*>(g)[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+            for (int hh = 0; hh < 64; hh += 32) {
+              uint32_t v[32];
+              tmem_ld32(acc + c + hh, v);
+              tc_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 32; j += 2)
+                o[(hh + j) / 2] = pack_bf16x2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]));
+            }
           }
-        } else if constexpr (OP == kDh) {
-          if (row < n) {
-            float* o = a.acc + ((int64_t)s * a.T + row) * a.K + n0 + c;
+          if (OP != kGrad && empty) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (c + j < cols) {
-                const float x = empty ? 0.f : __uint_as_float(v[j]);
-                o[j] = a.first ? x : o[j] + x;
-              }
+            for (int j = 0; j < 32; ++j) o[j] = 0u;
           }
-        } else {
-          if (row < a.nv) {
-            __nv_bfloat16* o = a.dw + (int64_t)(a.v0 + row) * a.lddw + n0 + c;
+          const uint32_t stage = out_smem + (out & 1) * kOutBytes;
+          if (threadIdx.x == 128) bulk_wait_read<1>();  // the store before last has left this buffer
+          epi_barrier();
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (c + j < cols) o[j] = f2bf(empty ? 0.f : __uint_as_float(v[j]));
+          for (int j = 0; j < 8; ++j)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + sw128_offset(r, 16 * j)), "r"(o[4 * j]),
+                         "r"(o[4 * j + 1]), "r"(o[4 * j + 2]), "r"(o[4 * j + 3])
+                         : "memory");
+          fence_proxy_async_smem();
+          epi_barrier();
+          if (threadIdx.x == 128) {
+            if (any_row) {  // a box that starts inside; what reaches past the end is not written
+              if constexpr (OP == kGrad) tma_store(&tmO, stage, n0 + c, m0);
+              else if constexpr (OP == kDw) tma_store(&tmO, stage, n0 + c, a.v0 + m0);
+              else if (a.first) tma_store(&tmO, stage, n0 + c, s * a.acc_rows + m0);
+              else tma_add_f32(&tmO, stage, n0 + c, s * a.acc_rows + m0);
+            }
+            bulk_commit();
           }
         }
-      }
-      tc_fence_before();
-      mbar_arrive(bar_tempty + 8 * buf);
-      if constexpr (OP == kStats) {
-        if (row < n) a.part[(int64_t)nn * a.T + row] = make_float2(mx, sum);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_cluster(release + 8 * buf);
       }
     }
+    if (OP != kStats && threadIdx.x == 128) bulk_wait_all();
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+  cluster_barrier();
   tc_fence_after();
-  if (warp == 2) tmem_dealloc(tmem, 512);
+  if (warp == 2) tmem_dealloc2(tmem, 512);
 }
 
 // ---------------------------------------------------------------------------
@@ -360,7 +477,7 @@ struct PrepArgs {
   int *count, *target, *token, *place;  // place: [T] row of hc, or -1
   float *zt, *loss;                     // loss: [T] by token (ignored rows: 0)
   unsigned* ticket;
-  int T, V, K, Kp, rows;
+  int T, V, K, Kp, rows, vec;  // vec: rows of h in whole 16-byte vectors (W's and hc's are)
   float cap, inv_cap;
 };
 
@@ -409,10 +526,21 @@ __global__ void __launch_bounds__(256) prep_kernel(PrepArgs a) {
     const __nv_bfloat16* wr = a.w + (valid ? y : 0) * a.ldw;
     __nv_bfloat16* o = a.hc + (int64_t)d * a.Kp;
     float s = 0.f;
-    for (int c = lane; c < a.Kp; c += 32) {
-      const __nv_bfloat16 x = c < a.K ? hr[c] : f2bf(0.f);
-      o[c] = x;
-      if (c < a.K) s = fmaf(bf2f(x), bf2f(wr[c]), s);
+    if (a.vec) {
+#pragma unroll 4
+      for (int c = lane * 8; c < a.K; c += 256) {
+        const uint4 hv = *reinterpret_cast<const uint4*>(hr + c), wv = *reinterpret_cast<const uint4*>(wr + c);
+        *reinterpret_cast<uint4*>(o + c) = hv;
+        const __nv_bfloat16 *he = reinterpret_cast<const __nv_bfloat16*>(&hv), *we = reinterpret_cast<const __nv_bfloat16*>(&wv);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s = fmaf(bf2f(he[j]), bf2f(we[j]), s);
+      }
+    } else {
+      for (int c = lane; c < a.Kp; c += 32) {
+        const __nv_bfloat16 x = c < a.K ? hr[c] : f2bf(0.f);
+        o[c] = x;
+        if (c < a.K) s = fmaf(bf2f(x), bf2f(wr[c]), s);
+      }
     }
     s = warp_sum(s);
     if (lane == 0) {
@@ -448,7 +576,7 @@ struct MergeArgs {
   unsigned* ticket;
   int T, nt, mean;
 };
-constexpr int kMergeWarps = 16;
+constexpr int kMergeWarps = 32;
 
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
   const float top = fmaxf(m, m2);
@@ -471,9 +599,15 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(MergeArgs a) {
   const int row = blockIdx.x * 32 + lane;
   float m = -INFINITY, s = 0.f;
   if (row < n)
-    for (int t = warp; t < a.nt; t += kMergeWarps) {
-      const float2 p = a.part[(int64_t)t * a.T + row];
-      join(m, s, p.x, p.y);
+    for (int t = warp; t < a.nt; t += 8 * kMergeWarps) {  // eight loads in flight
+      float2 p[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int q = t + i * kMergeWarps;
+        p[i] = q < a.nt ? a.part[(int64_t)q * a.T + row] : make_float2(-INFINITY, 0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) join(m, s, p[i].x, p[i].y);
     }
   sh[warp][lane] = make_float2(m, s);
   __syncthreads();
@@ -499,31 +633,72 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(MergeArgs a) {
   if (threadIdx.x == 0) *a.total = a.mean ? acc / (float)max(n, 1) : acc;
 }
 
-// dh[t] = sum over the contraction's parts of acc[.][place[t]], 0 for ignored rows.
-__global__ void __launch_bounds__(256) finish_dh_kernel(const float* acc, const int* place, __nv_bfloat16* dh, int T,
-                                                        int K, int splits) {
+// dh[t] = sum over the contraction's parts of acc[.][place[t]] + e W[y], 0 for
+// ignored rows. e is what the target's entry of G lost when it was rounded to bf16:
+// that entry alone is of the size of the whole row, the others are far below it, so
+// with it added back the rounding of G hardly shows in dh (measured against 64 bits:
+// 2.7e-3 -> 1.7e-3, the output's own rounding). A row a CTA.
+struct FinishArgs {
+  Args g;
+  const float* acc;
+  const int* place;
+  const __nv_bfloat16* w;
+  __nv_bfloat16* dh;
+  int64_t ldw;
+  int lda;  // row stride of acc
+};
+__global__ void __launch_bounds__(256) finish_dh_kernel(const FinishArgs a) {
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t total = (int64_t)T * K;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int t = (int)(i / K);
-    const int c = (int)(i - (int64_t)t * K);
-    const int p = place[t];
-    float s = 0.f;
-    if (p >= 0)
-      for (int k = 0; k < splits; ++k) s += acc[((int64_t)k * T + p) * K + c];
-    dh[i] = f2bf(s);
+  const int t = blockIdx.x, K = a.g.K;
+  const int p = a.place[t];
+  __nv_bfloat16* o = a.dh + (int64_t)t * K;
+  float e = 0.f;
+  const __nv_bfloat16* wr = a.w;
+  if (p >= 0) {
+    const float g = target_grad(a.g, p, 1.f / (float)max(*a.g.count, 1));
+    e = g - bf2f(f2bf(g));
+    wr += (int64_t)max(a.g.target[p], 0) * a.ldw;
+  }
+  const float* row = a.acc + (int64_t)max(p, 0) * a.lda;
+  const int64_t part = (int64_t)a.g.acc_rows * a.lda;
+  if (K % 8 == 0) {  // W's rows and acc's are 16-byte aligned whatever K is; dh's are if K is whole
+    for (int c = threadIdx.x * 8; c < K; c += 256 * 8) {
+      uint4 out = make_uint4(0, 0, 0, 0);
+      if (p >= 0) {
+        float s[8];
+        const uint4 wv = *reinterpret_cast<const uint4*>(wr + c);
+        const __nv_bfloat16* we = reinterpret_cast<const __nv_bfloat16*>(&wv);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] = e * bf2f(we[j]);
+        for (int k = 0; k < a.g.splits; ++k) {
+          const float4 x = *reinterpret_cast<const float4*>(row + k * part + c);
+          const float4 y = *reinterpret_cast<const float4*>(row + k * part + c + 4);
+          s[0] += x.x, s[1] += x.y, s[2] += x.z, s[3] += x.w;
+          s[4] += y.x, s[5] += y.y, s[6] += y.z, s[7] += y.w;
+        }
+        out = make_uint4(pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3]), pack_bf16x2(s[4], s[5]), pack_bf16x2(s[6], s[7]));
+      }
+      *reinterpret_cast<uint4*>(o + c) = out;
+    }
+  } else {
+    for (int c = threadIdx.x; c < K; c += 256) {
+      float s = p >= 0 ? e * bf2f(wr[c]) : 0.f;
+      if (p >= 0)
+        for (int k = 0; k < a.g.splits; ++k) s += row[k * part + c];
+      o[c] = f2bf(s);
+    }
   }
 }
 
 template <int OP>
-static int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const Args& a, int64_t tiles, int num_sms,
-                       cudaStream_t st) {
+static int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& to, const Args& a, int64_t tiles,
+                       int num_sms, cudaStream_t st) {
   if (tiles <= 0) return 0;
   if (tiles > 0x7FFFFFFFll - 1024) return -1;
   if (int e = smem_attr_once<gemm_kernel<OP>>(kSmem)) return e;
-  const int grid = (int)(tiles < num_sms ? tiles : num_sms);
-  cudaError_t e = launch_k(gemm_kernel<OP>, dim3(grid), dim3(kThreads), kSmem, st, 1, ta, tb, a);
+  const int grid = (int)(tiles < num_sms / 2 ? tiles : num_sms / 2);
+  cudaError_t e = launch_k(gemm_kernel<OP>, dim3(2 * grid), dim3(kThreads), kSmem, st, 1, ta, tb, to, a);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
@@ -537,14 +712,11 @@ using namespace b200::lce;
 
 extern "C" {
 
-// Workspace shapes. Column tiles of the statistics: ceil(V / 256).
-int b200_lce_tile_cols() { return kTileN; }
-
 // Parts of the contraction of dh for T rows of K columns: enough tiles for every
-// SM where the rows alone give too few (a part keeps 16 blocks of 64 or more).
+// pair of SMs where the rows alone give too few (a part keeps 16 blocks of 64 or more).
 int b200_lce_dh_splits(int T, int K, int piece, int num_sms) {
   const int64_t tiles = tiles_of(T, kTileM) * tiles_of(K, kTileN);
-  int64_t s = tiles ? num_sms / tiles : 1;
+  int64_t s = tiles ? num_sms / 2 / tiles : 1;
   const int64_t most = piece / 64 / 16;
   s = s > most ? most : s;
   return (int)(s > 64 ? 64 : s < 1 ? 1 : s);
@@ -581,6 +753,7 @@ int b200_lce_forward(const void* h, int64_t ldh, const void* W, int64_t ldw, con
   p.Kp = Kp;
   p.cap = cap;
   p.inv_cap = cap > 0.f ? 1.f / cap : 0.f;
+  p.vec = K % 8 == 0 && ldh % 8 == 0 && ((uintptr_t)h & 15) == 0;
   // eight rows a CTA (one a warp) while that is at most four CTAs an SM
   const int64_t want = tiles_of(T, 4 * num_sms);
   p.rows = (int)(want < 8 ? 8 : want > 8192 ? 8192 : (want + 7) / 8 * 8);
@@ -599,8 +772,8 @@ int b200_lce_forward(const void* h, int64_t ldh, const void* W, int64_t ldw, con
   a.cap = p.cap;
   a.inv_cap = p.inv_cap;
   CUtensorMap ta, tb;
-  if (!make_tmap_2d(&ta, hc, T, Kp, Kp, kTileM, 64, 2) || !make_tmap_2d(&tb, W, V, K, ldw, kTileN, 64, 2)) return -1;
-  if (int r = launch_gemm<kStats>(ta, tb, a, tiles_of(T, kTileM) * tiles_of(V, kTileN), num_sms, st)) return r;
+  if (!make_tmap_2d(&ta, hc, T, Kp, Kp, kRowsM, 64, 2) || !make_tmap_2d(&tb, W, V, K, ldw, kRowsN, 64, 2)) return -1;
+  if (int r = launch_gemm<kStats>(ta, tb, ta, a, tiles_of(T, kTileM) * tiles_of(V, kTileN), num_sms, st)) return r;
   MergeArgs g = {};
   g.part = a.part;
   g.count = p.count;
@@ -617,57 +790,70 @@ int b200_lce_forward(const void* h, int64_t ldh, const void* W, int64_t ldw, con
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
+// Rows and row stride (elements) of one part of dh's fp32 sums for T rows of K columns.
+int b200_lce_acc_rows(int T) { return (int)(tiles_of(T, kRowsM) * kRowsM); }
+int b200_lce_acc_cols(int K) { return (K + 3) / 4 * 4; }
+
 // Backward from the forward's hc, ints and floats. dloss: element token *
-// dloss_stride. dh [T, K] contiguous and dW [V, K] (row stride lddw) are null where
-// not wanted. piece: columns of the vocabulary at a time, a multiple of 256; G bf16
-// [T, piece]; acc fp32 [splits, T, K] for dh.
+// dloss_stride. dh [T, K] contiguous and dW [V, K] (row stride lddw, a multiple of
+// 8) are null where not wanted. piece: columns of the vocabulary at a time, a
+// multiple of 256; G bf16 [T, piece]; acc fp32 [splits, acc_rows, acc_cols] for dh.
 int b200_lce_backward(const void* hc, const void* W, int64_t ldw, const int* ints, const float* floats,
                       const float* dloss, int64_t dloss_stride, int mean, int T, int V, int K, int Kp, float cap,
                       int piece, void* G, float* acc, int splits, void* dh, void* dW, int64_t lddw, int num_sms,
                       cudaStream_t st) {
   if (T <= 0 || V <= 0 || K <= 0 || Kp < K || (Kp % 8) || (ldw % 8) || ((uintptr_t)W & 15) || piece <= 0 ||
-      (piece % kTileN) || splits < 1 || ((uintptr_t)G & 15) || (dh && !acc))
+      (piece % kTileN) || splits < 1 || ((uintptr_t)G & 15) || (dh && (!acc || ((uintptr_t)acc & 15) || ((uintptr_t)dh & 15))) ||
+      (dW && ((lddw % 8) || lddw < K || ((uintptr_t)dW & 15))) || (int64_t)splits * b200_lce_acc_rows(T) > 0x7FFFFFFFll)
     return -1;
   Args a = {};
   a.count = ints;
   a.target = ints + 2;
   a.token = ints + 2 + (int64_t)T;
-  const int* place = ints + 2 + 2 * (int64_t)T;
   a.zt = floats;
   a.loss = floats + T;
   a.dloss = dloss;
   a.dloss_stride = dloss_stride;
   a.mean = mean;
-  a.G = reinterpret_cast<__nv_bfloat16*>(G);
-  a.ldg = piece;
-  a.acc = acc;
-  a.dw = reinterpret_cast<__nv_bfloat16*>(dW);
-  a.lddw = lddw;
+  a.acc_rows = b200_lce_acc_rows(T);
   a.T = T;
   a.V = V;
   a.K = K;
   a.splits = splits;
   a.cap = cap;
   a.inv_cap = cap > 0.f ? 1.f / cap : 0.f;
-  CUtensorMap h_rows, w_rows, g_rows, w_cols, g_cols, h_cols;
-  if (!make_tmap_2d(&h_rows, hc, T, Kp, Kp, kTileM, 64, 2) || !make_tmap_2d(&w_rows, W, V, K, ldw, kTileN, 64, 2) ||
-      !make_tmap_2d(&g_rows, G, T, piece, piece, kTileM, 64, 2) || !make_tmap_2d(&w_cols, W, V, K, ldw, 64, 64, 2) ||
-      !make_tmap_2d(&g_cols, G, T, piece, piece, 64, 64, 2) || !make_tmap_2d(&h_cols, hc, T, Kp, Kp, 64, 64, 2))
+  const int lda = b200_lce_acc_cols(K);
+  CUtensorMap h_rows, w_rows, g_rows, w_cols, g_cols, h_cols, o_dh, o_dw;
+  if (!make_tmap_2d(&h_rows, hc, T, Kp, Kp, kRowsM, 64, 2) || !make_tmap_2d(&w_rows, W, V, K, ldw, kRowsN, 64, 2) ||
+      !make_tmap_2d(&g_rows, G, T, piece, piece, kRowsM, 64, 2))
+    return -1;
+  if (dh && (!make_tmap_2d(&w_cols, W, V, K, ldw, 64, 64, 2) ||
+             !make_tmap_2d(&o_dh, acc, (int64_t)splits * a.acc_rows, K, lda, kRowsM, 32, 4)))
+    return -1;
+  if (dW && (!make_tmap_2d(&g_cols, G, T, piece, piece, 64, 64, 2) || !make_tmap_2d(&h_cols, hc, T, Kp, Kp, 64, 64, 2) ||
+             !make_tmap_2d(&o_dw, dW, V, K, lddw, kRowsM, 64, 2)))
     return -1;
   for (int64_t v0 = 0; v0 < V; v0 += piece) {
     a.v0 = (int)v0;
     a.nv = (int)(V - v0 < piece ? V - v0 : piece);
     a.first = v0 == 0;
-    if (int r = launch_gemm<kGrad>(h_rows, w_rows, a, tiles_of(T, kTileM) * tiles_of(a.nv, kTileN), num_sms, st)) return r;
+    const int64_t rows = tiles_of(T, kTileM);
+    if (int r = launch_gemm<kGrad>(h_rows, w_rows, g_rows, a, rows * tiles_of(a.nv, kTileN), num_sms, st)) return r;
     if (dh)
-      if (int r = launch_gemm<kDh>(g_rows, w_cols, a, tiles_of(T, kTileM) * tiles_of(K, kTileN) * splits, num_sms, st)) return r;
+      if (int r = launch_gemm<kDh>(g_rows, w_cols, o_dh, a, rows * tiles_of(K, kTileN) * splits, num_sms, st)) return r;
     if (dW)
-      if (int r = launch_gemm<kDw>(g_cols, h_cols, a, tiles_of(a.nv, kTileM) * tiles_of(K, kTileN), num_sms, st)) return r;
+      if (int r = launch_gemm<kDw>(g_cols, h_cols, o_dw, a, tiles_of(a.nv, kTileM) * tiles_of(K, kTileN), num_sms, st)) return r;
   }
   if (dh) {
-    const int64_t blocks = tiles_of((int64_t)T * K, 256);
-    cudaError_t e = launch_k(finish_dh_kernel, dim3((unsigned)(blocks < 8 * num_sms ? blocks : 8 * num_sms)), dim3(256), 0,
-                             st, 1, acc, place, reinterpret_cast<__nv_bfloat16*>(dh), T, K, splits);
+    FinishArgs f = {};
+    f.g = a;
+    f.acc = acc;
+    f.place = ints + 2 + 2 * (int64_t)T;
+    f.w = reinterpret_cast<const __nv_bfloat16*>(W);
+    f.ldw = ldw;
+    f.dh = reinterpret_cast<__nv_bfloat16*>(dh);
+    f.lda = lda;
+    cudaError_t e = launch_k(finish_dh_kernel, dim3((unsigned)T), dim3(256), 0, st, 1, f);
     if (e != cudaSuccess) return (int)e;
   }
   return (int)cudaGetLastError();

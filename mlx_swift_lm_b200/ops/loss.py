@@ -15,7 +15,8 @@ from ._args import rows2d, same_device
 from .linear import num_sms
 
 _lib.register_signatures({
-    "b200_lce_tile_cols": (_lib.i32, []),
+    "b200_lce_acc_rows": (_lib.i32, [_lib.i32]),
+    "b200_lce_acc_cols": (_lib.i32, [_lib.i32]),
     "b200_lce_dh_splits": (_lib.i32, [_lib.i32, _lib.i32, _lib.i32, _lib.i32]),
     "b200_lce_forward": (_lib.i32, [_lib.vp, _lib.i64, _lib.vp, _lib.i64, _lib.vp, _lib.i64, _lib.i32, _lib.i32,
                                     _lib.i32, _lib.i32, _lib.f32, _lib.vp, _lib.vp, _lib.vp, _lib.vp, _lib.vp,
@@ -85,14 +86,15 @@ class _LinearCrossEntropy(torch.autograd.Function):
         L, sms = _lib.lib(), num_sms(dev)
         G = torch.empty((T, piece), dtype=torch.bfloat16, device=dev)
         dh = torch.empty((T, K), dtype=torch.bfloat16, device=dev) if need_h else None
-        dw = torch.empty((V, K), dtype=torch.bfloat16, device=dev) if need_w else None
+        dw = torch.empty((V, Kp), dtype=torch.bfloat16, device=dev)[:, :K] if need_w else None  # rows as TMA stores them
         splits = L.b200_lce_dh_splits(T, K, piece, sms)
-        acc = torch.empty((splits, T, K), dtype=torch.float32, device=dev) if need_h else None
+        acc = (torch.empty(splits * L.b200_lce_acc_rows(T) * L.b200_lce_acc_cols(K), dtype=torch.float32, device=dev)
+               if need_h else None)
         g = dloss.reshape(-1)
         rc = _lib.launch(L.b200_lce_backward, dev, hc.data_ptr(), w2.data_ptr(), w2.stride(0), ints.data_ptr(),
                          floats.data_ptr(), g.data_ptr(), g.stride(0) if g.numel() > 1 else 0, 1 if ctx.mean else 0, T,
                          V, K, Kp, ctx.softcap, piece, G.data_ptr(), _lib.ptr(acc), splits, _lib.ptr(dh),
-                         _lib.ptr(dw), K, sms)
+                         _lib.ptr(dw), Kp, sms)
         _lib.check(rc, f"linear_cross_entropy backward T={T} V={V} K={K}")
         _lib.count(-(-V // piece) * (1 + (dh is not None) + (dw is not None)) + (dh is not None))
         return dh, dw, None, None, None, None
