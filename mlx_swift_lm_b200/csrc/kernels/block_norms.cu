@@ -22,6 +22,8 @@
 // of a thread in turn, then a butterfly over 32 such groups, then one over the
 // group sums. It is the order of add_rmsnorm_kernel, whose results these equal
 // bit for bit.
+#include <type_traits>
+
 #include "b200_elem.cuh"
 
 namespace b200 {
@@ -41,77 +43,78 @@ struct BlockNormArgs {
   int64_t ldx, ldd, ldg, ldy, ldh, lddy, lddh, ldo;  // row strides; ldo: dx, ddelta and dgate
   int64_t T;
   int H;
-  int gate_kind, w_type;
+  int gate_kind;
   int want_post, want_pre, want_gate;
   int offset_one, round_branch;
   float eps, scale;
 };
 
-// Column of element j of a thread's v-th group of eight. Aligned rows: eight
-// neighbours (one 16- or 32-byte access); others: one column a lane, so that a
-// warp's access is contiguous.
-template <bool VEC>
+// Column of element j of a thread's v-th group of E. Aligned rows: E neighbours
+// (16- or 32-byte accesses); others: one column a lane, so that a warp's access is
+// contiguous.
+template <bool VEC, int E = 8>
 __device__ __forceinline__ int column(int v, int j, int threads) {
-  return VEC ? (v * threads + (int)threadIdx.x) * 8 + j : (v * 8 + j) * threads + (int)threadIdx.x;
+  return VEC ? (v * threads + (int)threadIdx.x) * E + j : (v * E + j) * threads + (int)threadIdx.x;
 }
 
-template <typename T, bool VEC>
-__device__ __forceinline__ Pack8<T> load_group(const T* row, int v, int threads, int H) {
-  Pack8<T> p;
+template <typename T, int E>
+struct alignas(sizeof(T) * E >= 16 ? 16 : sizeof(T) * E) Group {
+  T e[E];
+};
+
+template <typename T, bool VEC, int E = 8>
+__device__ __forceinline__ Group<T, E> load_group(const T* row, int v, int threads, int H) {
+  Group<T, E> p;
   if constexpr (VEC) {
-    const int c = column<true>(v, 0, threads);
-    if (c < H) return load_pack(row + c);
+    const int c = column<true, E>(v, 0, threads);
+    if (c < H) {
+      if constexpr (sizeof(p) >= 16) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) p.e[j] = from_f32<T>(0.f);
+        for (int i = 0; i < (int)(sizeof(p) / 16); ++i)
+          reinterpret_cast<uint4*>(&p)[i] = reinterpret_cast<const uint4*>(row + c)[i];
+      } else {
+        *reinterpret_cast<uint2*>(&p) = *reinterpret_cast<const uint2*>(row + c);
+      }
+      return p;
+    }
+#pragma unroll
+    for (int j = 0; j < E; ++j) p.e[j] = from_f32<T>(0.f);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = column<false>(v, j, threads);
+    for (int j = 0; j < E; ++j) {
+      const int c = column<false, E>(v, j, threads);
       p.e[j] = c < H ? row[c] : from_f32<T>(0.f);
     }
   }
   return p;
 }
-template <typename T, bool VEC>
-__device__ __forceinline__ void store_group(T* row, const Pack8<T>& p, int v, int threads, int H) {
+template <typename T, bool VEC, int E = 8>
+__device__ __forceinline__ void store_group(T* row, const Group<T, E>& p, int v, int threads, int H) {
   if constexpr (VEC) {
-    const int c = column<true>(v, 0, threads);
-    if (c < H) store_pack(row + c, p);
+    const int c = column<true, E>(v, 0, threads);
+    if (c < H) {
+      if constexpr (sizeof(p) >= 16) {
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(p) / 16); ++i)
+          reinterpret_cast<uint4*>(row + c)[i] = reinterpret_cast<const uint4*>(&p)[i];
+      } else {
+        *reinterpret_cast<uint2*>(row + c) = *reinterpret_cast<const uint2*>(&p);
+      }
+    }
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = column<false>(v, j, threads);
+    for (int j = 0; j < E; ++j) {
+      const int c = column<false, E>(v, j, threads);
       if (c < H) row[c] = p.e[j];
     }
   }
 }
-// Eight weights (0 past the row's end).
-template <bool VEC>
-__device__ __forceinline__ void load_weights(float* w, const void* p, int type, int v, int threads, int H) {
-  if (VEC && column<true>(v, 0, threads) < H) {
-    const int c = column<true>(v, 0, threads);
-    if (type == kElemF32) {
-      const Pack8<float> q = load_pack(reinterpret_cast<const float*>(p) + c);
+template <typename T, bool VEC, int E>
+__device__ __forceinline__ void weights_of(float* w, const void* p, int v, int threads, int H) {
+  const Group<T, E> q = load_group<T, VEC, E>(reinterpret_cast<const T*>(p), v, threads, H);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = q.e[j];
-    } else if (type == kElemBf16) {
-      const Pack8<__nv_bfloat16> q = load_pack(reinterpret_cast<const __nv_bfloat16*>(p) + c);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = to_f32(q.e[j]);
-    } else {
-      const Pack8<__half> q = load_pack(reinterpret_cast<const __half*>(p) + c);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = to_f32(q.e[j]);
-    }
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int c = column<VEC>(v, j, threads);
-    w[j] = !VEC && c < H ? load_elem(p, type, c) : 0.f;
-  }
+  for (int j = 0; j < E; ++j) w[j] = to_f32(q.e[j]);
 }
-
 // Sum over the block of NV group sums a thread: a butterfly over the lanes for
 // each group index, then one over the at most 32 warp sums, in index order.
 // `red`: 32 floats that no other reduction of the same row uses.
@@ -129,8 +132,8 @@ __device__ __forceinline__ float row_sum(const float (&s)[NV], float* red) {
 
 // One row a CTA. NV groups of eight a thread; SEQ: rows above 8192 columns add a
 // thread's groups one after the other, shorter ones sum each group on its own.
-template <typename T, bool VEC, int NV, bool SEQ>
-__global__ void __launch_bounds__(1024) block_norms_kernel(BlockNormArgs a) {
+template <typename T, typename W, bool VEC, int NV, bool SEQ>
+__global__ void __launch_bounds__(1024, 1) block_norms_kernel(BlockNormArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   __shared__ float red[2][32];
@@ -139,7 +142,7 @@ __global__ void __launch_bounds__(1024) block_norms_kernel(BlockNormArgs a) {
   const int n = blockDim.x, H = a.H;
   const T* xr = reinterpret_cast<const T*>(a.x) + row * a.ldx;
   const T* dr = reinterpret_cast<const T*>(a.delta) + row * a.ldd;
-  Pack8<T> x[NV], d[NV];
+  Group<T, 8> x[NV], d[NV];
 #pragma unroll
   for (int v = 0; v < NV; ++v) d[v] = load_group<T, VEC>(dr, v, n, H);
 #pragma unroll
@@ -163,13 +166,10 @@ __global__ void __launch_bounds__(1024) block_norms_kernel(BlockNormArgs a) {
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     float w[8], g[8];
-    if (a.post) load_weights<VEC>(w, a.post, a.w_type, v, n, H);
-    if (a.gate_kind == kGateChannel) load_weights<VEC>(g, a.gate, sizeof(T) == 4 ? kElemF32 : (std::is_same<T, __half>::value ? kElemF16 : kElemBf16), v, n, H);
-    if (a.gate_kind == kGateElement) {
-      const Pack8<T> q = load_group<T, VEC>(reinterpret_cast<const T*>(a.gate) + row * a.ldg, v, n, H);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) g[j] = to_f32(q.e[j]);
-    }
+    if (a.post) weights_of<W, VEC, 8>(w, a.post, v, n, H);
+    if (a.gate_kind == kGateChannel) weights_of<T, VEC, 8>(g, a.gate, v, n, H);
+    if (a.gate_kind == kGateElement)
+      weights_of<T, VEC, 8>(g, reinterpret_cast<const T*>(a.gate) + row * a.ldg, v, n, H);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       float u = to_f32(d[v].e[j]);
@@ -191,138 +191,180 @@ __global__ void __launch_bounds__(1024) block_norms_kernel(BlockNormArgs a) {
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     float w[8];
-    load_weights<VEC>(w, a.pre, a.w_type, v, n, H);
+    weights_of<W, VEC, 8>(w, a.pre, v, n, H);
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[v].e[j] = from_f32<T>(to_f32(x[v].e[j]) * r2 * (w[j] + one));
     store_group<T, VEC>(hr, x[v], v, n, H);
   }
 }
 
+// Three sums over the block in one round: red holds 3 x 32 floats.
+__device__ __forceinline__ void row_sums3(float& a, float& b, float& c, float (*red)[32]) {
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  a = warp_sum(a);
+  b = warp_sum(b);
+  c = warp_sum(c);
+  if (lane == 0) {
+    red[0][wid] = a;
+    red[1][wid] = b;
+    red[2][wid] = c;
+  }
+  __syncthreads();
+  const bool in = lane < nw;
+  a = warp_sum(in ? red[0][lane] : 0.f);
+  b = warp_sum(in ? red[1][lane] : 0.f);
+  c = warp_sum(in ? red[2][lane] : 0.f);
+}
+
 // Backward: a CTA walks the rows blockIdx.x, + gridDim.x, ... and keeps its
-// columns' weight-gradient sums in registers, so that they cost gridDim.x
-// partial rows instead of T. `part` is summed over the CTAs afterwards, in order.
+// columns' weight-gradient sums in registers, so that they cost gridDim.x partial
+// rows instead of T. `part` is summed over the CTAs afterwards, in order.
+//
+// Both means come from one round of sums: with c = gate * post * dhat and
+// b = dy + r2 g, mean(w * dhat) = scale * (sum c b - r2 m sum c yhat) / H where
+// m = mean(g * yhat), so neither waits for the other. Groups of four columns leave
+// registers for the next row's loads to be under way while this row's sums are taken.
+constexpr int kBwdE = 4;
+
 template <typename T, bool VEC, int NV>
-__global__ void __launch_bounds__(1024) block_norms_bwd_kernel(BlockNormArgs a) {
+struct BwdRow {
+  Group<T, kBwdE> y[NV], d[NV], ty[NV], th[NV];
+  __device__ __forceinline__ void load(const BlockNormArgs& a, int64_t row, int n) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      d[v] = load_group<T, VEC, kBwdE>(reinterpret_cast<const T*>(a.delta) + row * a.ldd, v, n, a.H);
+      if (a.dh) {
+        y[v] = load_group<T, VEC, kBwdE>(reinterpret_cast<const T*>(a.y) + row * a.ldy, v, n, a.H);
+        th[v] = load_group<T, VEC, kBwdE>(reinterpret_cast<const T*>(a.dh) + row * a.lddh, v, n, a.H);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kBwdE; ++j) y[v].e[j] = th[v].e[j] = from_f32<T>(0.f);
+      }
+      if (a.dy) {
+        ty[v] = load_group<T, VEC, kBwdE>(reinterpret_cast<const T*>(a.dy) + row * a.lddy, v, n, a.H);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kBwdE; ++j) ty[v].e[j] = from_f32<T>(0.f);
+      }
+    }
+  }
+};
+// Weights as factors: 1 without post, 0 without dh (whose rows are zeros then too).
+template <typename W, bool VEC>
+__device__ __forceinline__ void factors(float* w, const void* p, float one, float none, int v, int n, int H) {
+  if (p) {
+    weights_of<W, VEC, kBwdE>(w, p, v, n, H);
+#pragma unroll
+    for (int j = 0; j < kBwdE; ++j) w[j] += one;
+  } else {
+#pragma unroll
+    for (int j = 0; j < kBwdE; ++j) w[j] = none;
+  }
+}
+
+template <typename T, typename W, bool VEC, int NV, bool GATED>
+__global__ void __launch_bounds__(1024, 1) block_norms_bwd_kernel(const BlockNormArgs a) {
+  constexpr int E = kBwdE;
   pdl_launch_dependents();
   pdl_wait();
   __shared__ float red[2][3][32];
   const int n = blockDim.x, H = a.H;
-  const float one = a.offset_one ? 1.f : 0.f;
-  float cpost[NV][8] = {}, cpre[NV][8] = {}, cgate[NV][8] = {};
-  constexpr int kT = sizeof(T) == 4 ? kElemF32 : (std::is_same<T, __half>::value ? kElemF16 : kElemBf16);
+  const float one = a.offset_one ? 1.f : 0.f, inv_h = 1.f / (float)H;
+  const void* pre = a.dh ? a.pre : nullptr;
+  float cpost[NV][E] = {}, cpre[NV][E] = {}, cgate[GATED ? NV : 1][E] = {};
   int flip = 0;
+  BwdRow<T, VEC, NV> in;
+  if ((int64_t)blockIdx.x < a.T) in.load(a, blockIdx.x, n);
   for (int64_t row = blockIdx.x; row < a.T; row += gridDim.x, flip ^= 1) {
-    // the reductions' buffers alternate between rows: a thread may be writing the
-    // next row's sums while a slower one still reads this row's
-    Pack8<T> y[NV], d[NV], ty[NV], th[NV];
+    // the sums' buffers alternate between rows: a thread may be writing the next
+    // row's while a slower one still reads this row's
+    const float r1 = a.post ? a.r1[row] : 1.f, r2 = a.dh ? a.r2[row] : 0.f;
+    const float grow = GATED && a.gate_kind == kGateRow ? to_f32(reinterpret_cast<const T*>(a.gate)[row]) : 1.f;
+    const void* gate = nullptr;  // a gate along the columns
+    if (GATED && a.gate_kind == kGateChannel) gate = a.gate;
+    if (GATED && a.gate_kind == kGateElement) gate = reinterpret_cast<const T*>(a.gate) + row * a.ldg;
+    float s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      if (a.dh) {
-        y[v] = load_group<T, VEC>(reinterpret_cast<const T*>(a.y) + row * a.ldy, v, n, H);
-        th[v] = load_group<T, VEC>(reinterpret_cast<const T*>(a.dh) + row * a.lddh, v, n, H);
+      float wq[E], wp[E], g[E];
+      factors<W, VEC>(wq, pre, one, 0.f, v, n, H);
+      factors<W, VEC>(wp, a.post, one, 1.f, v, n, H);
+      if (GATED) factors<T, VEC>(g, gate, 0.f, 1.f, v, n, H);
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const float yh = to_f32(in.y[v].e[j]) * r2, t = to_f32(in.th[v].e[j]);
+        float c = to_f32(in.d[v].e[j]) * r1 * wp[j];
+        if (GATED) c *= g[j];
+        const float gq = t * wq[j];
+        cpre[v][j] += t * yh;
+        s1 += gq * yh;
+        s2 += c * (to_f32(in.ty[v].e[j]) + r2 * gq);
+        s3 += c * yh;
       }
-      if (a.dy) ty[v] = load_group<T, VEC>(reinterpret_cast<const T*>(a.dy) + row * a.lddy, v, n, H);
-      d[v] = load_group<T, VEC>(reinterpret_cast<const T*>(a.delta) + row * a.ldd, v, n, H);
     }
-    float dt[NV][8];
-    if (a.dh) {
-      const float r2 = a.r2[row];
-      float s[1] = {0.f};
-#pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        float w[8];
-        load_weights<VEC>(w, a.pre, a.w_type, v, n, H);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float yh = to_f32(y[v].e[j]) * r2, g = to_f32(th[v].e[j]);
-          cpre[v][j] += g * yh;
-          dt[v][j] = g * (w[j] + one);
-          s[0] += dt[v][j] * yh;
-        }
-      }
-      const float m = row_sum(s, red[flip][0]) / (float)H;
-#pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          dt[v][j] = r2 * (dt[v][j] - to_f32(y[v].e[j]) * r2 * m) + (a.dy ? to_f32(ty[v].e[j]) : 0.f);
-    } else {
-#pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) dt[v][j] = a.dy ? to_f32(ty[v].e[j]) : 0.f;
-    }
-    T* dxr = reinterpret_cast<T*>(a.dx) + row * a.ldo;
-    const float r1 = a.post ? a.r1[row] : 1.f;
-    const float grow = a.gate_kind == kGateRow ? to_f32(reinterpret_cast<const T*>(a.gate)[row]) : 1.f;
-    float s[1] = {0.f}, sg[1] = {0.f};
+    BwdRow<T, VEC, NV> cur = in;
+    if (NV <= 2 && row + gridDim.x < a.T) in.load(a, row + gridDim.x, n);
+    row_sums3(s1, s2, s3, red[flip]);
+    const float m = r2 * s1 * inv_h;              // dt = b - m yhat
+    const float along = a.scale * (s2 - m * s3);  // sum of scale * dt * c, without a row gate
+    const float m1 = a.post ? along * grow * inv_h : 0.f;
+    if (GATED && a.gate_kind == kGateRow && a.dgate && threadIdx.x == 0)
+      reinterpret_cast<T*>(a.dgate)[row] = from_f32<T>(along);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      if (a.dx) {
-        Pack8<T> o;
+      float wq[E], wp[E], g[E];
+      factors<W, VEC>(wq, pre, one, 0.f, v, n, H);
+      factors<W, VEC>(wp, a.post, one, 1.f, v, n, H);
+      if (GATED) factors<T, VEC>(g, gate, 0.f, 1.f, v, n, H);
+      Group<T, E> ox, od, og;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o.e[j] = from_f32<T>(dt[v][j]);
-        store_group<T, VEC>(dxr, o, v, n, H);
-      }
-      float w[8], g[8];
-      if (a.post) load_weights<VEC>(w, a.post, a.w_type, v, n, H);
-      if (a.gate_kind == kGateChannel) load_weights<VEC>(g, a.gate, kT, v, n, H);
-      if (a.gate_kind == kGateElement) {
-        const Pack8<T> q = load_group<T, VEC>(reinterpret_cast<const T*>(a.gate) + row * a.ldg, v, n, H);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] = to_f32(q.e[j]);
-      }
-      Pack8<T> og;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float dhat = to_f32(d[v].e[j]) * r1;
-        const float wj = a.post ? w[j] + one : 1.f;
-        float du = a.scale * dt[v][j];
-        if (a.gate_kind != kGateNone) {
-          const float dg = du * dhat * wj;
+      for (int j = 0; j < E; ++j) {
+        const float dt = to_f32(cur.ty[v].e[j]) + r2 * (to_f32(cur.th[v].e[j]) * wq[j]) - to_f32(cur.y[v].e[j]) * r2 * m;
+        const float dhat = to_f32(cur.d[v].e[j]) * r1;
+        float du = a.scale * dt;
+        if (GATED) {
+          const float dg = du * dhat * wp[j];
           cgate[v][j] += dg;
-          sg[0] += dg;
           og.e[j] = from_f32<T>(dg);
-          du *= a.gate_kind == kGateRow ? grow : g[j];
+          du *= g[j] * grow;
         }
         cpost[v][j] += du * dhat;
-        dt[v][j] = du * wj;  // gradient of dhat
-        s[0] += dt[v][j] * dhat;
+        ox.e[j] = from_f32<T>(dt);
+        od.e[j] = from_f32<T>(r1 * (du * wp[j] - dhat * m1));
       }
-      if (a.gate_kind == kGateElement && a.dgate)
-        store_group<T, VEC>(reinterpret_cast<T*>(a.dgate) + row * a.ldo, og, v, n, H);
+      if (a.dx) store_group<T, VEC, E>(reinterpret_cast<T*>(a.dx) + row * a.ldo, ox, v, n, H);
+      if (a.ddelta) store_group<T, VEC, E>(reinterpret_cast<T*>(a.ddelta) + row * a.ldo, od, v, n, H);
+      if (GATED && a.gate_kind == kGateElement && a.dgate)
+        store_group<T, VEC, E>(reinterpret_cast<T*>(a.dgate) + row * a.ldo, og, v, n, H);
     }
-    if (a.gate_kind == kGateRow && a.dgate) {
-      const float t = row_sum(sg, red[flip][1]);
-      if (threadIdx.x == 0) reinterpret_cast<T*>(a.dgate)[row] = from_f32<T>(t);
-    }
-    if (a.ddelta) {
-      const float m = a.post ? row_sum(s, red[flip][2]) / (float)H : 0.f;
-      T* ddr = reinterpret_cast<T*>(a.ddelta) + row * a.ldo;
-#pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        Pack8<T> o;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o.e[j] = from_f32<T>(r1 * (dt[v][j] - to_f32(d[v].e[j]) * r1 * m));
-        store_group<T, VEC>(ddr, o, v, n, H);
-      }
-    }
+    if (NV > 2 && row + gridDim.x < a.T) in.load(a, row + gridDim.x, n);
   }
   float* part = a.part;
-  auto put = [&](const float (&c)[NV][8]) {
+  auto put = [&](const float (&c)[E], int v) {
     float* r = part + (int64_t)blockIdx.x * H;
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int col = column<VEC>(v, j, n);
-        if (col < H) r[col] = c[v][j];
-      }
-    part += (int64_t)gridDim.x * H;
+    for (int j = 0; j < E; ++j) {
+      const int col = column<VEC, E>(v, j, n);
+      if (col < H) r[col] = c[j];
+    }
   };
-  if (a.want_post) put(cpost);
-  if (a.want_pre) put(cpre);
-  if (a.want_gate && a.gate_kind == kGateChannel) put(cgate);
+  const int64_t next = (int64_t)gridDim.x * H;
+  if (a.want_post) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) put(cpost[v], v);
+    part += next;
+  }
+  if (a.want_pre) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) put(cpre[v], v);
+    part += next;
+  }
+  if constexpr (GATED) {
+    if (a.want_gate && a.gate_kind == kGateChannel) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) put(cgate[v], v);
+    }
+  }
 }
 
 struct ColSumArgs {
@@ -353,33 +395,58 @@ __global__ void __launch_bounds__(1024) col_sum_kernel(ColSumArgs a) {
 
 static inline int round32(int v) { return (v + 31) / 32 * 32; }
 
-template <typename T, bool VEC>
-static int launch_fwd(const BlockNormArgs& a, cudaStream_t st) {
+// Groups of eight a thread, forward. Rows above 8192 columns need more than one for
+// each of 1024 threads. Below, one keeps a few rows' latency low and four leave room
+// for eight times the rows on an SM, whose loads then overlap the others' sums
+// (8192 x 4096 bf16: see kFewRows); both add in the same order. Unaligned rows are
+// dealt to the lanes by the thread count, so there the choice goes by the width alone.
+constexpr int kFewRows = 4;  // rows an SM
+template <typename T, typename W, bool VEC>
+static int launch_fwd(const BlockNormArgs& a, int num_sms, cudaStream_t st) {
   const int groups = (a.H + 7) / 8;
-  const int full = round32(groups < 1024 ? groups : 1024);  // threads at one group each
   const dim3 grid((unsigned)a.T);
   cudaError_t e;
-  if (groups > 2048)
-    e = launch_k(block_norms_kernel<T, VEC, 4, true>, grid, dim3(1024), 0, st, 1, a);
-  else if (groups > 1024)
-    e = launch_k(block_norms_kernel<T, VEC, 2, true>, grid, dim3(1024), 0, st, 1, a);
+  if (groups > 1024)
+    e = launch_k(block_norms_kernel<T, W, VEC, 4, true>, grid, dim3(1024), 0, st, 1, a);
+  else if (VEC && a.T <= (int64_t)kFewRows * num_sms)
+    e = launch_k(block_norms_kernel<T, W, VEC, 1, false>, grid, dim3(round32(groups)), 0, st, 1, a);
   else
-    e = launch_k(block_norms_kernel<T, VEC, 1, false>, grid, dim3(full), 0, st, 1, a);
+    e = launch_k(block_norms_kernel<T, W, VEC, 4, false>, grid, dim3(round32((groups + 3) / 4)), 0, st, 1, a);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
-template <typename T, bool VEC>
-static int launch_bwd(const BlockNormArgs& a, int grid, cudaStream_t st) {
-  const int groups = (a.H + 7) / 8;
-  const int full = round32(groups < 1024 ? groups : 1024);
+static inline int bwd_groups(int H) { return (H + kBwdE - 1) / kBwdE; }
+static inline int bwd_threads(int H) {
+  const int g = bwd_groups(H);
+  return round32(g < 1024 ? g : 1024);
+}
+
+template <typename T, typename W, bool VEC, bool GATED>
+static int launch_bwd_gate(const BlockNormArgs& a, int grid, cudaStream_t st) {
+  const int groups = bwd_groups(a.H);
+  const dim3 threads(bwd_threads(a.H));
   cudaError_t e;
   if (groups > 2048)
-    e = launch_k(block_norms_bwd_kernel<T, VEC, 4>, dim3(grid), dim3(1024), 0, st, 1, a);
+    e = launch_k(block_norms_bwd_kernel<T, W, VEC, 8, GATED>, dim3(grid), threads, 0, st, 1, a);
   else if (groups > 1024)
-    e = launch_k(block_norms_bwd_kernel<T, VEC, 2>, dim3(grid), dim3(1024), 0, st, 1, a);
+    e = launch_k(block_norms_bwd_kernel<T, W, VEC, 2, GATED>, dim3(grid), threads, 0, st, 1, a);
   else
-    e = launch_k(block_norms_bwd_kernel<T, VEC, 1>, dim3(grid), dim3(full), 0, st, 1, a);
+    e = launch_k(block_norms_bwd_kernel<T, W, VEC, 1, GATED>, dim3(grid), threads, 0, st, 1, a);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
+}
+template <typename T, typename W, bool VEC>
+static int launch_bwd(const BlockNormArgs& a, int grid, cudaStream_t st) {
+  return a.gate_kind == kGateNone ? launch_bwd_gate<T, W, VEC, false>(a, grid, st)
+                                  : launch_bwd_gate<T, W, VEC, true>(a, grid, st);
+}
+
+// f(T, W, VEC) for the element type, the weights' type (that or fp32) and alignment.
+template <typename F>
+static int by_type(int type, int w_type, bool vec, F f) {
+  auto pick = [&](auto t, auto w) { return vec ? f(t, w, std::true_type{}) : f(t, w, std::false_type{}); };
+  if (type == kElemF32) return pick(float{}, float{});
+  if (type == kElemBf16) return w_type == kElemF32 ? pick(__nv_bfloat16{}, float{}) : pick(__nv_bfloat16{}, __nv_bfloat16{});
+  return w_type == kElemF32 ? pick(__half{}, float{}) : pick(__half{}, __half{});
 }
 
 }  // namespace b200
@@ -391,23 +458,23 @@ extern "C" {
 // Widest row: four groups of eight columns for each of 1024 threads.
 int b200_block_norms_max_width() { return 4 * 1024 * 8; }
 
-// CTAs of the backward pass (rows of its partial sums) for T rows of H columns.
+// CTAs of the backward pass (rows of its partial sums) for T rows of H columns: what
+// fits on the SMs at 64 registers a thread.
 int b200_block_norms_bwd_grid(int64_t T, int H, int num_sms) {
-  const int threads = round32((H + 7) / 8 < 1024 ? (H + 7) / 8 : 1024);
-  int per_sm = 1024 / threads;
+  int per_sm = 1024 / bwd_threads(H);
   per_sm = per_sm > 16 ? 16 : per_sm < 1 ? 1 : per_sm;
   const int64_t most = (int64_t)per_sm * num_sms;
   return (int)(T < most ? T : most);
 }
 
-// Forward. type: ElemType of x, delta, gate, y and h; w_type: of post and pre.
+// Forward. type: ElemType of x, delta, gate, y and h; w_type: of post and pre, that or fp32.
 // y may be x. Returns 0, a CUDA error code, or -1 for arguments out of range.
 int b200_block_norms(const void* x, int64_t ldx, const void* delta, int64_t ldd, const void* post, const void* pre,
                      int w_type, const void* gate, int64_t ldg, int gate_kind, void* y, int64_t ldy, void* h,
                      int64_t ldh, float* r1, float* r2, int64_t T, int H, int type, float eps, float scale,
-                     int offset_one, int round_branch, cudaStream_t st) {
+                     int offset_one, int round_branch, int num_sms, cudaStream_t st) {
   if (T < 0 || H < 1 || H > b200_block_norms_max_width() || T > 0x7FFFFFFFll || type < 0 || type > 2 || w_type < 0 ||
-      w_type > 2 || gate_kind < 0 || gate_kind > 3 || (gate_kind && !gate))
+      w_type > 2 || (w_type != type && w_type != kElemF32) || gate_kind < 0 || gate_kind > 3 || (gate_kind && !gate))
     return -1;
   if (T == 0) return 0;
   BlockNormArgs a = {};
@@ -428,7 +495,6 @@ int b200_block_norms(const void* x, int64_t ldx, const void* delta, int64_t ldd,
   a.T = T;
   a.H = H;
   a.gate_kind = gate_kind;
-  a.w_type = w_type;
   a.eps = eps;
   a.scale = scale;
   a.offset_one = offset_one;
@@ -437,9 +503,9 @@ int b200_block_norms(const void* x, int64_t ldx, const void* delta, int64_t ldd,
   auto rows16 = [&](const void* p, int64_t ld) { return (((uintptr_t)p | (uintptr_t)(ld * size)) & 15) == 0; };
   const bool vec = H % 8 == 0 && rows16(x, ldx) && rows16(delta, ldd) && rows16(y, ldy) && rows16(h, ldh) &&
                    rows16(post, 0) && rows16(pre, 0) && (gate_kind == kGateRow || rows16(gate, gate_kind == kGateElement ? ldg : 0));
-  if (type == kElemBf16) return vec ? launch_fwd<__nv_bfloat16, true>(a, st) : launch_fwd<__nv_bfloat16, false>(a, st);
-  if (type == kElemF16) return vec ? launch_fwd<__half, true>(a, st) : launch_fwd<__half, false>(a, st);
-  return vec ? launch_fwd<float, true>(a, st) : launch_fwd<float, false>(a, st);
+  return by_type(type, w_type, vec, [&](auto t, auto w, auto v) {
+    return launch_fwd<decltype(t), decltype(w), decltype(v)::value>(a, num_sms, st);
+  });
 }
 
 // Backward from y, delta and the saved r1 / r2. dy or dh may be null (zero); dx,
@@ -452,7 +518,7 @@ int b200_block_norms_bwd(const void* y, int64_t ldy, const void* delta, int64_t 
                          void* dgate, void* dpost, void* dpre, float* part, int64_t T, int H, int type, float scale,
                          int offset_one, int num_sms, cudaStream_t st) {
   if (T < 0 || H < 1 || H > b200_block_norms_max_width() || T > 0x7FFFFFFFll || type < 0 || type > 2 || w_type < 0 ||
-      w_type > 2 || gate_kind < 0 || gate_kind > 3 || (gate_kind && !gate) || (dh && !pre) || (dpre && !dh))
+      w_type > 2 || (w_type != type && w_type != kElemF32) || gate_kind < 0 || gate_kind > 3 || (gate_kind && !gate) || (dh && !pre) || (dpre && !dh))
     return -1;
   if (T == 0) return 0;
   BlockNormArgs a = {};
@@ -478,7 +544,6 @@ int b200_block_norms_bwd(const void* y, int64_t ldy, const void* delta, int64_t 
   a.T = T;
   a.H = H;
   a.gate_kind = gate_kind;
-  a.w_type = w_type;
   a.scale = scale;
   a.offset_one = offset_one;
   a.want_post = dpost != nullptr;
@@ -491,10 +556,9 @@ int b200_block_norms_bwd(const void* y, int64_t ldy, const void* delta, int64_t 
                    (gate_kind == kGateRow ||
                     (rows16(gate, gate_kind == kGateElement ? ldg : 0) && (gate_kind != kGateElement || rows16(dgate, 0))));
   const int grid = b200_block_norms_bwd_grid(T, H, num_sms);
-  int e;
-  if (type == kElemBf16) e = vec ? launch_bwd<__nv_bfloat16, true>(a, grid, st) : launch_bwd<__nv_bfloat16, false>(a, grid, st);
-  else if (type == kElemF16) e = vec ? launch_bwd<__half, true>(a, grid, st) : launch_bwd<__half, false>(a, grid, st);
-  else e = vec ? launch_bwd<float, true>(a, grid, st) : launch_bwd<float, false>(a, grid, st);
+  const int e = by_type(type, w_type, vec, [&](auto t, auto w, auto v) {
+    return launch_bwd<decltype(t), decltype(w), decltype(v)::value>(a, grid, st);
+  });
   if (e) return e;
   ColSumArgs c = {};
   int k = 0;

@@ -43,30 +43,41 @@ __device__ __forceinline__ unsigned keep_bits(const DropoutArgs& a, unsigned row
   return bits;
 }
 
-// Aligned rows: a thread owns a unit, 16-byte loads and stores.
+// Aligned rows: a thread owns two units at a time (16-byte loads and stores, both
+// under way before the first is drawn).
+constexpr int kUnits = 2;
 template <typename T>
-__global__ void __launch_bounds__(256) dropout_vec_kernel(DropoutArgs a) {
+__global__ void __launch_bounds__(256) dropout_vec_kernel(const DropoutArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   const uint64_t offset = a.offset + (a.offset_ptr ? (uint64_t)*a.offset_ptr : 0ull);
   const T* x = reinterpret_cast<const T*>(a.x);
   const T* res = reinterpret_cast<const T*>(a.residual);
   T* y = reinterpret_cast<T*>(a.y);
-  for (unsigned u = blockIdx.x * 256u + threadIdx.x; u < a.units; u += gridDim.x * 256u) {
-    const unsigned row = (unsigned)(((uint64_t)u * a.div_mul) >> a.div_shift);
-    const unsigned unit = u - row * a.units_per_row;
-    const int64_t r = row, c = (int64_t)unit * 8;
-    Pack8<T> v = load_pack(x + r * a.ldx + c);
-    Pack8<T> q;
-    if (res) q = load_pack(res + r * a.ldr + c);
-    const unsigned bits = keep_bits(a, a.row0 + row, unit, offset);
+  for (unsigned u0 = blockIdx.x * (256u * kUnits) + threadIdx.x; u0 < a.units; u0 += gridDim.x * (256u * kUnits)) {
+    Pack8<T> v[kUnits], q[kUnits];
+    unsigned row[kUnits], unit[kUnits];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float f = (bits >> j) & 1u ? to_f32(v.e[j]) * a.scale : 0.f;
-      if (res) f += to_f32(q.e[j]);
-      v.e[j] = from_f32<T>(f);
+    for (int i = 0; i < kUnits; ++i) {
+      const unsigned u = u0 + 256u * i;
+      row[i] = (unsigned)(((uint64_t)u * a.div_mul) >> a.div_shift);
+      unit[i] = u - row[i] * a.units_per_row;
+      if (u < a.units) {
+        v[i] = load_pack(x + (int64_t)row[i] * a.ldx + (int64_t)unit[i] * 8);
+        if (res) q[i] = load_pack(res + (int64_t)row[i] * a.ldr + (int64_t)unit[i] * 8);
+      }
     }
-    store_pack(y + r * a.ldy + c, v);
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      const unsigned bits = keep_bits(a, a.row0 + row[i], unit[i], offset);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float f = (bits >> j) & 1u ? to_f32(v[i].e[j]) * a.scale : 0.f;
+        if (res) f += to_f32(q[i].e[j]);
+        v[i].e[j] = from_f32<T>(f);
+      }
+      if (u0 + 256u * i < a.units) store_pack(y + (int64_t)row[i] * a.ldy + (int64_t)unit[i] * 8, v[i]);
+    }
   }
 }
 
@@ -74,7 +85,7 @@ __global__ void __launch_bounds__(256) dropout_vec_kernel(DropoutArgs a) {
 // draws one unit's bits; the elements then go by column = lane + 32 j, so that
 // every access of the warp is contiguous, with the bits fetched from their lane.
 template <typename T>
-__global__ void __launch_bounds__(256) dropout_any_kernel(DropoutArgs a) {
+__global__ void __launch_bounds__(256) dropout_any_kernel(const DropoutArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   const uint64_t offset = a.offset + (a.offset_ptr ? (uint64_t)*a.offset_ptr : 0ull);
@@ -131,9 +142,9 @@ static int launch_dropout(DropoutArgs a, int64_t rows, bool vec, int num_sms, cu
     a.y = y + r0 * a.ldy * (int64_t)sizeof(T);
     a.row0 = (unsigned)r0;
     a.units = (unsigned)(n * upr);
-    const unsigned per = vec ? 256 : 8;
+    const unsigned per = vec ? 256 * kUnits : 8;
     unsigned grid = (a.units + per - 1) / per;
-    const unsigned most = (unsigned)num_sms * 8;  // 2048 threads an SM
+    const unsigned most = (unsigned)num_sms * 8;  // no more CTAs than can be resident
     grid = grid < most ? grid : most;
     cudaError_t e = vec ? launch_k(dropout_vec_kernel<T>, dim3(grid), dim3(256), 0, st, 1, a)
                         : launch_k(dropout_any_kernel<T>, dim3(grid), dim3(256), 0, st, 1, a);

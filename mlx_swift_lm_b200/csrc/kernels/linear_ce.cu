@@ -59,7 +59,8 @@ struct Args {
   int acc_rows;          // kDh: rows of one part of the fp32 sums (whole half tiles, so that none reaches into the next)
   int T, V, K;
   int v0, nv;            // the piece's first column and columns
-  int splits, first;     // kDh: parts of the contraction; first piece stores, others add
+  int piece, pairs;      // kDh: columns of a whole piece and CTA pairs (choose_parts)
+  int most_parts, first;  // kDh: parts the sums have room for; first piece stores, others add
   float cap, inv_cap;    // cap 0: none
 };
 
@@ -149,6 +150,26 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Parts of dh's contraction of `kb` blocks of 64 over `tiles` output tiles: the
+// fewest that (nearly) minimise the rounds of the pairs times their length, so that
+// few rows still fill the machine and the last round is not half empty. A part costs
+// about kPartBlocks blocks beyond its product (its tile's way out). Chosen on the
+// device, where the number of scored rows is known.
+constexpr int kPartBlocks = 6;
+__host__ __device__ inline int choose_parts(int tiles, int kb, int pairs, int most) {
+  int best = 1;
+  int64_t cost = INT64_MAX;
+  for (int s = 1; s <= most && (s == 1 || kb / s >= 16); ++s) {
+    const int64_t rounds = ((int64_t)tiles * s + pairs - 1) / pairs;
+    const int64_t c = rounds * ((kb + s - 1) / s + kPartBlocks);
+    if (c < cost) {
+      cost = c;
+      best = s;
+    }
+  }
+  return best;
+}
+
 // The tile walk of one launch: `mt` x `nt` tiles (times `splits` of the
 // contraction), columns of kGroupM row tiles.
 struct Walk {
@@ -168,6 +189,12 @@ struct Walk {
 __device__ __forceinline__ float target_grad(const Args& a, int row, float inv_n) {
   const float q = a.zt[row] * a.inv_cap;  // inv_cap 0: no cap
   return expm1f(-a.loss[row]) * (1.f - q * q) * a.dloss[a.dloss_stride * a.token[row]] * (a.mean ? inv_n : 1.f);
+}
+
+// All pieces (the last may be shorter) and the final sum use the same parts.
+__device__ __forceinline__ int dh_parts(const Args& a, int n) {
+  const int tiles = ((n + kTileM - 1) / kTileM) * ((a.K + kTileN - 1) / kTileN);
+  return choose_parts(tiles, min(a.piece, a.V) / 64, a.pairs, a.most_parts);
 }
 
 template <int OP>
@@ -228,7 +255,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     w.nt = (a.K + kTileN - 1) / kTileN;
     kb_total = (n + 63) / 64;
   }
-  w.splits = OP == kDh ? a.splits : 1;
+  w.splits = OP == kDh ? dh_parts(a, n) : 1;
   w.total = w.mt * w.nt * w.splits;
   const int kb_per = (kb_total + w.splits - 1) / w.splits;
 
@@ -662,6 +689,7 @@ __global__ void __launch_bounds__(256) finish_dh_kernel(const FinishArgs a) {
   }
   const float* row = a.acc + (int64_t)max(p, 0) * a.lda;
   const int64_t part = (int64_t)a.g.acc_rows * a.lda;
+  const int parts = dh_parts(a.g, *a.g.count);
   if (K % 8 == 0) {  // W's rows and acc's are 16-byte aligned whatever K is; dh's are if K is whole
     for (int c = threadIdx.x * 8; c < K; c += 256 * 8) {
       uint4 out = make_uint4(0, 0, 0, 0);
@@ -671,7 +699,7 @@ __global__ void __launch_bounds__(256) finish_dh_kernel(const FinishArgs a) {
         const __nv_bfloat16* we = reinterpret_cast<const __nv_bfloat16*>(&wv);
 #pragma unroll
         for (int j = 0; j < 8; ++j) s[j] = e * bf2f(we[j]);
-        for (int k = 0; k < a.g.splits; ++k) {
+        for (int k = 0; k < parts; ++k) {
           const float4 x = *reinterpret_cast<const float4*>(row + k * part + c);
           const float4 y = *reinterpret_cast<const float4*>(row + k * part + c + 4);
           s[0] += x.x, s[1] += x.y, s[2] += x.z, s[3] += x.w;
@@ -685,7 +713,7 @@ __global__ void __launch_bounds__(256) finish_dh_kernel(const FinishArgs a) {
     for (int c = threadIdx.x; c < K; c += 256) {
       float s = p >= 0 ? e * bf2f(wr[c]) : 0.f;
       if (p >= 0)
-        for (int k = 0; k < a.g.splits; ++k) s += row[k * part + c];
+        for (int k = 0; k < parts; ++k) s += row[k * part + c];
       o[c] = f2bf(s);
     }
   }
@@ -712,26 +740,54 @@ using namespace b200::lce;
 
 extern "C" {
 
-// Parts of the contraction of dh for T rows of K columns: enough tiles for every
-// pair of SMs where the rows alone give too few (a part keeps 16 blocks of 64 or more).
-int b200_lce_dh_splits(int T, int K, int piece, int num_sms) {
-  const int64_t tiles = tiles_of(T, kTileM) * tiles_of(K, kTileN);
-  int64_t s = tiles ? num_sms / 2 / tiles : 1;
-  const int64_t most = piece / 64 / 16;
-  s = s > most ? most : s;
+// What a forward pass leaves for its backward pass, in one buffer of
+// b200_lce_saved_bytes: hc [T, Kp] bf16, then zt and row loss fp32 [T] each, then
+// int32 count, ticket, target [T], token [T], place [T].
+int64_t b200_lce_saved_bytes(int T, int Kp) { return (int64_t)T * Kp * 2 + ((int64_t)5 * T + 2) * 4; }
+
+// Scratch of the forward pass: a (max, sum) pair per row and column tile.
+int64_t b200_lce_forward_bytes(int T, int V) { return (int64_t)T * tiles_of(V, kTileN) * 8; }
+
+// Parts of dh's sums there is room for with up to T scored rows: eight rounds of tiles
+// of all CTA pairs, at most 155 MB, and always one.
+static int most_parts(int T, int K, int num_sms) {
+  const int64_t s = 8 * (num_sms / 2) / (tiles_of(T, kTileM) * tiles_of(K, kTileN));
   return (int)(s > 64 ? 64 : s < 1 ? 1 : s);
 }
+// Rows and row stride (elements) of one part of dh's sums.
+static int acc_rows(int T) { return (int)(tiles_of(T, kRowsM) * kRowsM); }
+static int acc_cols(int K) { return (K + 3) / 4 * 4; }
+
+// Scratch of the backward pass: one piece of G (bf16 [T, piece]), then dh's sums.
+int64_t b200_lce_backward_bytes(int T, int K, int piece, int want_dh, int num_sms) {
+  return (int64_t)T * piece * 2 + (want_dh ? (int64_t)most_parts(T, K, num_sms) * acc_rows(T) * acc_cols(K) * 4 : 0);
+}
+
+struct Saved {
+  uint8_t* hc;
+  float *zt, *loss;
+  int *count, *target, *token, *place;
+  Saved(void* p, int T, int Kp) {
+    hc = reinterpret_cast<uint8_t*>(p);
+    zt = reinterpret_cast<float*>(hc + (int64_t)T * Kp * 2);
+    loss = zt + T;
+    count = reinterpret_cast<int*>(loss + T);
+    target = count + 2;
+    token = target + T;
+    place = token + T;
+  }
+};
 
 // Forward. h [T, K] and W [V, K] bf16 (strides in elements; W 16-byte aligned with
-// ldw % 8 == 0), targets int64. hc [T, Kp], ints [3 T + 2] (count, ticket, target,
-// token, place), floats [2 T] (zt, row loss), part fp32 [2 ceil(V / 256) T]; loss
-// [T]; total [1] or null (mean: divided by the scored rows, at least 1).
-// Returns 0, a CUDA error code, or -1 for arguments out of range.
+// ldw % 8 == 0), targets int64. loss fp32 [T]; total [1] or null (mean: divided by
+// the scored rows, at least 1). Returns 0, a CUDA error code, or -1 for arguments
+// out of range.
 int b200_lce_forward(const void* h, int64_t ldh, const void* W, int64_t ldw, const int64_t* targets, int64_t ignore,
-                     int T, int V, int K, int Kp, float cap, void* hc, int* ints, float* floats, float* part,
-                     float* loss, float* total, int mean, int num_sms, cudaStream_t st) {
-  if (T <= 0 || V <= 0 || K <= 0 || Kp < K || (Kp % 8) || (ldw % 8) || ((uintptr_t)W & 15) || ((uintptr_t)hc & 15))
+                     int T, int V, int K, int Kp, float cap, void* saved, void* part, float* loss, float* total,
+                     int mean, int num_sms, cudaStream_t st) {
+  if (T <= 0 || V <= 0 || K <= 0 || Kp < K || (Kp % 8) || (ldw % 8) || ((uintptr_t)W & 15) || ((uintptr_t)saved & 15))
     return -1;
+  const Saved f(saved, T, Kp);
   PrepArgs p = {};
   p.h = reinterpret_cast<const __nv_bfloat16*>(h);
   p.w = reinterpret_cast<const __nv_bfloat16*>(W);
@@ -739,13 +795,13 @@ int b200_lce_forward(const void* h, int64_t ldh, const void* W, int64_t ldw, con
   p.ldh = ldh;
   p.ldw = ldw;
   p.ignore = ignore;
-  p.hc = reinterpret_cast<__nv_bfloat16*>(hc);
-  p.count = ints;
-  p.ticket = reinterpret_cast<unsigned*>(ints + 1);
-  p.target = ints + 2;
-  p.token = ints + 2 + (int64_t)T;
-  p.place = ints + 2 + 2 * (int64_t)T;
-  p.zt = floats;
+  p.hc = reinterpret_cast<__nv_bfloat16*>(f.hc);
+  p.count = f.count;
+  p.ticket = reinterpret_cast<unsigned*>(f.count + 1);
+  p.target = f.target;
+  p.token = f.token;
+  p.place = f.place;
+  p.zt = f.zt;
   p.loss = loss;
   p.T = T;
   p.V = V;
@@ -760,10 +816,10 @@ int b200_lce_forward(const void* h, int64_t ldh, const void* W, int64_t ldw, con
   cudaError_t e = launch_k(prep_kernel, dim3((unsigned)tiles_of(T, p.rows)), dim3(256), (p.rows + 1) * sizeof(int), st, 1, p);
   if (e != cudaSuccess) return (int)e;
   Args a = {};
-  a.count = p.count;
-  a.target = p.target;
-  a.token = p.token;
-  a.zt = p.zt;
+  a.count = f.count;
+  a.target = f.target;
+  a.token = f.token;
+  a.zt = f.zt;
   a.part = reinterpret_cast<float2*>(part);
   a.T = T;
   a.V = V;
@@ -772,14 +828,14 @@ int b200_lce_forward(const void* h, int64_t ldh, const void* W, int64_t ldw, con
   a.cap = p.cap;
   a.inv_cap = p.inv_cap;
   CUtensorMap ta, tb;
-  if (!make_tmap_2d(&ta, hc, T, Kp, Kp, kRowsM, 64, 2) || !make_tmap_2d(&tb, W, V, K, ldw, kRowsN, 64, 2)) return -1;
+  if (!make_tmap_2d(&ta, f.hc, T, Kp, Kp, kRowsM, 64, 2) || !make_tmap_2d(&tb, W, V, K, ldw, kRowsN, 64, 2)) return -1;
   if (int r = launch_gemm<kStats>(ta, tb, ta, a, tiles_of(T, kTileM) * tiles_of(V, kTileN), num_sms, st)) return r;
   MergeArgs g = {};
   g.part = a.part;
-  g.count = p.count;
-  g.token = p.token;
-  g.zt = p.zt;
-  g.row_loss = floats + T;
+  g.count = f.count;
+  g.token = f.token;
+  g.zt = f.zt;
+  g.row_loss = f.loss;
   g.loss = loss;
   g.total = total;
   g.ticket = p.ticket;
@@ -790,47 +846,47 @@ int b200_lce_forward(const void* h, int64_t ldh, const void* W, int64_t ldw, con
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
-// Rows and row stride (elements) of one part of dh's fp32 sums for T rows of K columns.
-int b200_lce_acc_rows(int T) { return (int)(tiles_of(T, kRowsM) * kRowsM); }
-int b200_lce_acc_cols(int K) { return (K + 3) / 4 * 4; }
-
-// Backward from the forward's hc, ints and floats. dloss: element token *
-// dloss_stride. dh [T, K] contiguous and dW [V, K] (row stride lddw, a multiple of
-// 8) are null where not wanted. piece: columns of the vocabulary at a time, a
-// multiple of 256; G bf16 [T, piece]; acc fp32 [splits, acc_rows, acc_cols] for dh.
-int b200_lce_backward(const void* hc, const void* W, int64_t ldw, const int* ints, const float* floats,
-                      const float* dloss, int64_t dloss_stride, int mean, int T, int V, int K, int Kp, float cap,
-                      int piece, void* G, float* acc, int splits, void* dh, void* dW, int64_t lddw, int num_sms,
-                      cudaStream_t st) {
+// Backward from what the forward pass saved. dloss: element token * dloss_stride.
+// dh [T, K] contiguous and dW [V, K] (row stride lddw, a multiple of 8) are null
+// where not wanted. piece: columns of the vocabulary at a time, a multiple of 256.
+int b200_lce_backward(void* saved, const void* W, int64_t ldw, const float* dloss, int64_t dloss_stride, int mean, int T,
+                      int V, int K, int Kp, float cap, int piece, void* scratch, void* dh, void* dW, int64_t lddw,
+                      int num_sms, cudaStream_t st) {
   if (T <= 0 || V <= 0 || K <= 0 || Kp < K || (Kp % 8) || (ldw % 8) || ((uintptr_t)W & 15) || piece <= 0 ||
-      (piece % kTileN) || splits < 1 || ((uintptr_t)G & 15) || (dh && (!acc || ((uintptr_t)acc & 15) || ((uintptr_t)dh & 15))) ||
-      (dW && ((lddw % 8) || lddw < K || ((uintptr_t)dW & 15))) || (int64_t)splits * b200_lce_acc_rows(T) > 0x7FFFFFFFll)
+      (piece % kTileN) || (((uintptr_t)saved | (uintptr_t)scratch | (uintptr_t)dh | (uintptr_t)dW) & 15) ||
+      (dW && ((lddw % 8) || lddw < K)))
     return -1;
+  const Saved f(saved, T, Kp);
   Args a = {};
-  a.count = ints;
-  a.target = ints + 2;
-  a.token = ints + 2 + (int64_t)T;
-  a.zt = floats;
-  a.loss = floats + T;
+  a.count = f.count;
+  a.target = f.target;
+  a.token = f.token;
+  a.zt = f.zt;
+  a.loss = f.loss;
   a.dloss = dloss;
   a.dloss_stride = dloss_stride;
   a.mean = mean;
-  a.acc_rows = b200_lce_acc_rows(T);
+  a.acc_rows = acc_rows(T);
   a.T = T;
   a.V = V;
   a.K = K;
-  a.splits = splits;
+  a.piece = piece;
+  a.pairs = num_sms / 2;
+  a.most_parts = most_parts(T, K, num_sms);
   a.cap = cap;
   a.inv_cap = cap > 0.f ? 1.f / cap : 0.f;
-  const int lda = b200_lce_acc_cols(K);
+  void* G = scratch;
+  float* acc = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(scratch) + (int64_t)T * piece * 2);
+  const int lda = acc_cols(K);
+  if ((int64_t)a.most_parts * a.acc_rows > 0x7FFFFFFFll) return -1;
   CUtensorMap h_rows, w_rows, g_rows, w_cols, g_cols, h_cols, o_dh, o_dw;
-  if (!make_tmap_2d(&h_rows, hc, T, Kp, Kp, kRowsM, 64, 2) || !make_tmap_2d(&w_rows, W, V, K, ldw, kRowsN, 64, 2) ||
+  if (!make_tmap_2d(&h_rows, f.hc, T, Kp, Kp, kRowsM, 64, 2) || !make_tmap_2d(&w_rows, W, V, K, ldw, kRowsN, 64, 2) ||
       !make_tmap_2d(&g_rows, G, T, piece, piece, kRowsM, 64, 2))
     return -1;
   if (dh && (!make_tmap_2d(&w_cols, W, V, K, ldw, 64, 64, 2) ||
-             !make_tmap_2d(&o_dh, acc, (int64_t)splits * a.acc_rows, K, lda, kRowsM, 32, 4)))
+             !make_tmap_2d(&o_dh, acc, (int64_t)a.most_parts * a.acc_rows, K, lda, kRowsM, 32, 4)))
     return -1;
-  if (dW && (!make_tmap_2d(&g_cols, G, T, piece, piece, 64, 64, 2) || !make_tmap_2d(&h_cols, hc, T, Kp, Kp, 64, 64, 2) ||
+  if (dW && (!make_tmap_2d(&g_cols, G, T, piece, piece, 64, 64, 2) || !make_tmap_2d(&h_cols, f.hc, T, Kp, Kp, 64, 64, 2) ||
              !make_tmap_2d(&o_dw, dW, V, K, lddw, kRowsM, 64, 2)))
     return -1;
   for (int64_t v0 = 0; v0 < V; v0 += piece) {
@@ -840,20 +896,20 @@ int b200_lce_backward(const void* hc, const void* W, int64_t ldw, const int* int
     const int64_t rows = tiles_of(T, kTileM);
     if (int r = launch_gemm<kGrad>(h_rows, w_rows, g_rows, a, rows * tiles_of(a.nv, kTileN), num_sms, st)) return r;
     if (dh)
-      if (int r = launch_gemm<kDh>(g_rows, w_cols, o_dh, a, rows * tiles_of(K, kTileN) * splits, num_sms, st)) return r;
+      if (int r = launch_gemm<kDh>(g_rows, w_cols, o_dh, a, rows * tiles_of(K, kTileN) * a.most_parts, num_sms, st)) return r;
     if (dW)
       if (int r = launch_gemm<kDw>(g_cols, h_cols, o_dw, a, tiles_of(a.nv, kTileM) * tiles_of(K, kTileN), num_sms, st)) return r;
   }
   if (dh) {
-    FinishArgs f = {};
-    f.g = a;
-    f.acc = acc;
-    f.place = ints + 2 + 2 * (int64_t)T;
-    f.w = reinterpret_cast<const __nv_bfloat16*>(W);
-    f.ldw = ldw;
-    f.dh = reinterpret_cast<__nv_bfloat16*>(dh);
-    f.lda = lda;
-    cudaError_t e = launch_k(finish_dh_kernel, dim3((unsigned)T), dim3(256), 0, st, 1, f);
+    FinishArgs q = {};
+    q.g = a;
+    q.acc = acc;
+    q.place = f.place;
+    q.w = reinterpret_cast<const __nv_bfloat16*>(W);
+    q.ldw = ldw;
+    q.dh = reinterpret_cast<__nv_bfloat16*>(dh);
+    q.lda = lda;
+    cudaError_t e = launch_k(finish_dh_kernel, dim3((unsigned)T), dim3(256), 0, st, 1, q);
     if (e != cudaSuccess) return (int)e;
   }
   return (int)cudaGetLastError();

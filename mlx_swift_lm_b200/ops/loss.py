@@ -15,15 +15,15 @@ from ._args import rows2d, same_device
 from .linear import num_sms
 
 _lib.register_signatures({
-    "b200_lce_acc_rows": (_lib.i32, [_lib.i32]),
-    "b200_lce_acc_cols": (_lib.i32, [_lib.i32]),
-    "b200_lce_dh_splits": (_lib.i32, [_lib.i32, _lib.i32, _lib.i32, _lib.i32]),
+    "b200_lce_saved_bytes": (_lib.i64, [_lib.i32, _lib.i32]),
+    "b200_lce_forward_bytes": (_lib.i64, [_lib.i32, _lib.i32]),
+    "b200_lce_backward_bytes": (_lib.i64, [_lib.i32, _lib.i32, _lib.i32, _lib.i32, _lib.i32]),
     "b200_lce_forward": (_lib.i32, [_lib.vp, _lib.i64, _lib.vp, _lib.i64, _lib.vp, _lib.i64, _lib.i32, _lib.i32,
-                                    _lib.i32, _lib.i32, _lib.f32, _lib.vp, _lib.vp, _lib.vp, _lib.vp, _lib.vp,
-                                    _lib.vp, _lib.i32, _lib.i32, _lib.vp]),
-    "b200_lce_backward": (_lib.i32, [_lib.vp, _lib.vp, _lib.i64, _lib.vp, _lib.vp, _lib.vp, _lib.i64, _lib.i32,
-                                     _lib.i32, _lib.i32, _lib.i32, _lib.i32, _lib.f32, _lib.i32, _lib.vp, _lib.vp,
-                                     _lib.i32, _lib.vp, _lib.vp, _lib.i64, _lib.i32, _lib.vp]),
+                                    _lib.i32, _lib.i32, _lib.f32, _lib.vp, _lib.vp, _lib.vp, _lib.vp, _lib.i32,
+                                    _lib.i32, _lib.vp]),
+    "b200_lce_backward": (_lib.i32, [_lib.vp, _lib.vp, _lib.i64, _lib.vp, _lib.i64, _lib.i32, _lib.i32, _lib.i32,
+                                     _lib.i32, _lib.i32, _lib.f32, _lib.i32, _lib.vp, _lib.vp, _lib.vp, _lib.i64,
+                                     _lib.i32, _lib.vp]),
 }, status_tags=("linear_ce",))
 
 _TILE = 256  # columns of a tile; pieces of the vocabulary are whole tiles
@@ -45,58 +45,54 @@ def _aligned_head(w: torch.Tensor) -> torch.Tensor:
 
 
 def _forward(h2, w, targets, softcap, ignore_index, reduction):
+    """(losses or their total, what the backward pass needs)."""
     T, K = h2.shape
     V = w.shape[0]
     Kp = (K + 7) // 8 * 8
     dev = h2.device
     w = _aligned_head(w)
-    hc = torch.empty((T, Kp), dtype=torch.bfloat16, device=dev)
-    ints = torch.empty(3 * T + 2, dtype=torch.int32, device=dev)
-    floats = torch.empty(2 * T, dtype=torch.float32, device=dev)
-    part = torch.empty(2 * T * ((V + _TILE - 1) // _TILE), dtype=torch.float32, device=dev)
+    L = _lib.lib()
+    saved = torch.empty(L.b200_lce_saved_bytes(T, Kp), dtype=torch.uint8, device=dev)
+    part = torch.empty(L.b200_lce_forward_bytes(T, V), dtype=torch.uint8, device=dev)
     loss = torch.empty(T, dtype=torch.float32, device=dev)
     total = None if reduction == "none" else torch.empty((), dtype=torch.float32, device=dev)
-    rc = _lib.launch(_lib.lib().b200_lce_forward, dev, h2.data_ptr(), h2.stride(0), w.data_ptr(), w.stride(0),
-                     targets.data_ptr(), ignore_index, T, V, K, Kp, softcap, hc.data_ptr(), ints.data_ptr(),
-                     floats.data_ptr(), part.data_ptr(), loss.data_ptr(), _lib.ptr(total),
-                     1 if reduction == "mean" else 0, num_sms(dev))
+    rc = _lib.launch(L.b200_lce_forward, dev, h2.data_ptr(), h2.stride(0), w.data_ptr(), w.stride(0),
+                     targets.data_ptr(), ignore_index, T, V, K, Kp, softcap, saved.data_ptr(), part.data_ptr(),
+                     loss.data_ptr(), _lib.ptr(total), 1 if reduction == "mean" else 0, num_sms(dev))
     _lib.check(rc, f"linear_cross_entropy T={T} V={V} K={K}")
     _lib.count(3)
-    return loss if total is None else total, hc, ints, floats
+    return loss if total is None else total, saved
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h2, w, targets, softcap, ignore_index, reduction):
-        out, hc, ints, floats = _forward(h2, w, targets, softcap, ignore_index, reduction)
-        ctx.save_for_backward(w, hc, ints, floats)
+        out, saved = _forward(h2, w, targets, softcap, ignore_index, reduction)
+        ctx.save_for_backward(w, saved)
         ctx.shape, ctx.softcap, ctx.mean = h2.shape, softcap, reduction == "mean"
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
-        w, hc, ints, floats = ctx.saved_tensors
+        w, saved = ctx.saved_tensors
         (T, K), (V, _), dev = ctx.shape, w.shape, w.device
         need_h, need_w = ctx.needs_input_grad[:2]
-        Kp = hc.shape[1]
+        Kp = (K + 7) // 8 * 8
         w2 = _aligned_head(w)
         piece = max(MIN_PIECE, PIECE_BYTES // (2 * T) // _TILE * _TILE)
         piece = min(piece, (V + _TILE - 1) // _TILE * _TILE)
         L, sms = _lib.lib(), num_sms(dev)
-        G = torch.empty((T, piece), dtype=torch.bfloat16, device=dev)
+        scratch = torch.empty(L.b200_lce_backward_bytes(T, K, piece, 1 if need_h else 0, sms), dtype=torch.uint8,
+                              device=dev)
         dh = torch.empty((T, K), dtype=torch.bfloat16, device=dev) if need_h else None
         dw = torch.empty((V, Kp), dtype=torch.bfloat16, device=dev)[:, :K] if need_w else None  # rows as TMA stores them
-        splits = L.b200_lce_dh_splits(T, K, piece, sms)
-        acc = (torch.empty(splits * L.b200_lce_acc_rows(T) * L.b200_lce_acc_cols(K), dtype=torch.float32, device=dev)
-               if need_h else None)
         g = dloss.reshape(-1)
-        rc = _lib.launch(L.b200_lce_backward, dev, hc.data_ptr(), w2.data_ptr(), w2.stride(0), ints.data_ptr(),
-                         floats.data_ptr(), g.data_ptr(), g.stride(0) if g.numel() > 1 else 0, 1 if ctx.mean else 0, T,
-                         V, K, Kp, ctx.softcap, piece, G.data_ptr(), _lib.ptr(acc), splits, _lib.ptr(dh),
-                         _lib.ptr(dw), Kp, sms)
+        rc = _lib.launch(L.b200_lce_backward, dev, saved.data_ptr(), w2.data_ptr(), w2.stride(0), g.data_ptr(),
+                         g.stride(0) if T > 1 and g.numel() == T else 0, 1 if ctx.mean else 0, T, V, K, Kp, ctx.softcap,
+                         piece, scratch.data_ptr(), _lib.ptr(dh), _lib.ptr(dw), Kp, sms)
         _lib.check(rc, f"linear_cross_entropy backward T={T} V={V} K={K}")
-        _lib.count(-(-V // piece) * (1 + (dh is not None) + (dw is not None)) + (dh is not None))
+        _lib.count(-(-V // piece) * (1 + need_h + need_w) + need_h)
         return dh, dw, None, None, None, None
 
 

@@ -12,7 +12,7 @@ from .linear import num_sms
 _lib.register_signatures({
     "b200_block_norms": (_lib.i32, [_lib.vp, _lib.i64, _lib.vp, _lib.i64, _lib.vp, _lib.vp, _lib.i32, _lib.vp, _lib.i64,
                                     _lib.i32, _lib.vp, _lib.i64, _lib.vp, _lib.i64, _lib.vp, _lib.vp, _lib.i64,
-                                    _lib.i32, _lib.i32, _lib.f32, _lib.f32, _lib.i32, _lib.i32, _lib.vp]),
+                                    _lib.i32, _lib.i32, _lib.f32, _lib.f32, _lib.i32, _lib.i32, _lib.i32, _lib.vp]),
     "b200_block_norms_bwd": (_lib.i32, [_lib.vp, _lib.i64, _lib.vp, _lib.i64, _lib.vp, _lib.vp, _lib.i32, _lib.vp,
                                         _lib.i64, _lib.i32, _lib.vp, _lib.vp, _lib.vp, _lib.i64, _lib.vp, _lib.i64,
                                         _lib.vp, _lib.vp, _lib.vp, _lib.vp, _lib.vp, _lib.vp, _lib.i64, _lib.i32,
@@ -106,10 +106,10 @@ def _block_norms_fwd(x, delta, post_w, pre_w, gate, kind, eps, scale, offset_one
     if T:
         rc = _lib.launch(
             _lib.lib().b200_block_norms, dev, x2.data_ptr(), x2.stride(0), d2.data_ptr(), d2.stride(0),
-            _lib.ptr(post_w), _lib.ptr(pre_w), 0 if w is None else ELEM[w.dtype], _lib.ptr(g),
+            _lib.ptr(post_w), _lib.ptr(pre_w), ELEM[x.dtype if w is None else w.dtype], _lib.ptr(g),
             g.stride(0) if kind == _GATE_ELEMENT else 0, kind, y2.data_ptr(), y2.stride(0), _lib.ptr(h), H,
             _lib.ptr(r1), _lib.ptr(r2), T, H, ELEM[x.dtype], float(eps), float(scale), 1 if offset_one else 0,
-            1 if round_branch else 0)
+            1 if round_branch else 0, num_sms(dev))
         _lib.check(rc, "block_norms")
         _lib.count(1)
     return y, h, r1, r2
@@ -158,7 +158,7 @@ class _BlockNorms(torch.autograd.Function):
                 if n_part else None)
         rc = _lib.launch(
             L.b200_block_norms_bwd, dev, y2.data_ptr(), y2.stride(0), d2.data_ptr(), d2.stride(0), _lib.ptr(pw),
-            _lib.ptr(qw), 0 if w is None else ELEM[w.dtype], _lib.ptr(g), g.stride(0) if kind == _GATE_ELEMENT else 0,
+            _lib.ptr(qw), ELEM[y.dtype if w is None else w.dtype], _lib.ptr(g), g.stride(0) if kind == _GATE_ELEMENT else 0,
             kind, _lib.ptr(r1), _lib.ptr(r2), _lib.ptr(dy2), 0 if dy2 is None else dy2.stride(0), _lib.ptr(dh2),
             0 if dh2 is None else dh2.stride(0), _lib.ptr(dx), _lib.ptr(dd), _lib.ptr(dgate), _lib.ptr(dpost),
             _lib.ptr(dpre), _lib.ptr(part), T, H, ELEM[y.dtype], ctx.scale, 1 if ctx.offset_one else 0, sms)
@@ -178,7 +178,7 @@ def block_norms(x: torch.Tensor, delta: torch.Tensor, post_w: torch.Tensor | Non
 
     Returns (y, h), differentiable in x, delta, the weights and the gate. x and
     delta [..., H] (bf16, fp16 or fp32, H up to 32768); gate of x's dtype with
-    shape [H], [..., 1] or [..., H]; post_w and pre_w [H] of one dtype.
+    shape [H], [..., 1] or [..., H]; post_w and pre_w [H] of one dtype, x's or fp32.
     `offset_one`: the weights are stored minus one. `round_branch`: u is rounded
     to x's dtype before the gate, as a separate norm and add would (bit-equal to
     ``add_rmsnorm(x, rmsnorm(delta, post_w), pre_w)``). `inplace`: y is written
@@ -196,8 +196,8 @@ def block_norms(x: torch.Tensor, delta: torch.Tensor, post_w: torch.Tensor | Non
     for w in (post_w, pre_w):
         if w is not None and w.shape != (H,):
             raise ValueError(f"block_norms: weight {tuple(w.shape)} for rows of {H}")
-        if w is not None:
-            elem_code(w, "block_norms weight")
+        if w is not None and w.dtype != x.dtype and w.dtype != torch.float32:
+            raise TypeError(f"block_norms: weight {w.dtype} for x {x.dtype}")
     if post_w is not None and pre_w is not None and post_w.dtype != pre_w.dtype:
         raise TypeError(f"block_norms: post_w {post_w.dtype}, pre_w {pre_w.dtype}")
     same_device("block_norms", x, delta, post_w, pre_w, gate)
