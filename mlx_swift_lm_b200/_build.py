@@ -1,6 +1,6 @@
 """In-tree build of the native parts of the framework.
 
-Two shared objects are produced under ``mlx_swift_lm_b200/_lib/``:
+Three shared objects are produced under ``mlx_swift_lm_b200/_lib/``:
 
 * ``libb200kernels.so`` - every CUDA kernel in ``csrc/kernels/*.cu``, compiled
   for sm_100a only (``-gencode arch=compute_100a,code=sm_100a``) and exposed
@@ -8,6 +8,8 @@ Two shared objects are produced under ``mlx_swift_lm_b200/_lib/``:
   ``libb200kernels_checked.so`` is the same library built with
   ``-DB200_CHECKED=1`` (extra bounds checks that record a status code
   instead of trapping); ``B200LM_CHECKED=1`` loads it instead.
+* ``_b200torch*.so`` - the autograd nodes of the training operators in
+  ``csrc/torch/*.cpp``, against torch's headers.
 * ``_b200host*.so`` - the host runtime in ``csrc/host/*.cpp`` (page pool, block
   hasher, grammar engine, safetensors reader) as a pybind11
   module.
@@ -33,6 +35,7 @@ KERNEL_SO = os.path.join(LIBDIR, "libb200kernels.so")
 # bounds-checked variant (-DB200_CHECKED=1), loaded with B200LM_CHECKED=1
 KERNEL_SO_CHECKED = os.path.join(LIBDIR, "libb200kernels_checked.so")
 OBJDIR_CHECKED = os.path.join(LIBDIR, "obj_checked")
+TORCH_SO = os.path.join(LIBDIR, "_b200torch" + sysconfig.get_config_var("EXT_SUFFIX"))
 HOST_SO = os.path.join(LIBDIR, "_b200host" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
@@ -104,6 +107,29 @@ def build_host(verbose: bool = False) -> str:
     return HOST_SO
 
 
+def build_torch(verbose: bool = False) -> str:
+    """The autograd module. Its kernels' addresses are given to it at run time, so it
+    links torch only."""
+    sources = sorted(glob.glob(os.path.join(CSRC, "torch", "*.cpp")))
+    if not _newer(sources + [os.path.join(CSRC, "include", "b200_train.h")], TORCH_SO):
+        return TORCH_SO
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    cuda = os.path.dirname(os.path.dirname(NVCC))
+    inc = ["-isystem" + p for p in include_paths() + [os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]]
+    os.makedirs(LIBDIR, exist_ok=True)
+    cmd = (["g++"] + CXX_FLAGS + [f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                                  "-DTORCH_EXTENSION_NAME=_b200torch", "-I" + os.path.join(CSRC, "include")]
+           + inc + sources + ["-o", TORCH_SO] + ["-L" + p for p in library_paths()]
+           + ["-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python",
+              "-L" + os.path.join(cuda, "lib64"), "-lcudart"])
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    _run(cmd)
+    return TORCH_SO
+
+
 def build_host_sanitized(outdir: str, sanitizer: str = "address,undefined") -> str:
     """The host module built with ``-fsanitize=<sanitizer>`` into `outdir`
     (same module name, so a process that puts `outdir` first on sys.path and
@@ -121,14 +147,16 @@ def build_host_sanitized(outdir: str, sanitizer: str = "address,undefined") -> s
 
 
 def build_all(verbose: bool = False, checked: bool = True) -> None:
-    """Release kernels, the host module, and (unless `checked` is False) the
+    """Release kernels, the host and autograd modules, and (unless `checked` is False) the
     bounds-checked kernel variant."""
-    with cf.ThreadPoolExecutor(max_workers=3) as ex:
+    with cf.ThreadPoolExecutor(max_workers=4) as ex:
         fk = ex.submit(build_kernels, verbose)
         fh = ex.submit(build_host, verbose)
+        ft = ex.submit(build_torch, verbose)
         fc = ex.submit(build_kernels, verbose, None, True) if checked else None
         fk.result()
         fh.result()
+        ft.result()
         if fc is not None:
             fc.result()
 
@@ -137,3 +165,4 @@ if __name__ == "__main__":
     build_all(verbose="-v" in sys.argv)
     print(KERNEL_SO)
     print(HOST_SO)
+    print(TORCH_SO)

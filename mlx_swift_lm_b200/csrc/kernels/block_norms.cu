@@ -22,9 +22,8 @@
 // of a thread in turn, then a butterfly over 32 such groups, then one over the
 // group sums. It is the order of add_rmsnorm_kernel, whose results these equal
 // bit for bit.
-#include <type_traits>
-
 #include "b200_elem.cuh"
+#include "b200_train.h"
 
 namespace b200 {
 
@@ -52,33 +51,16 @@ struct BlockNormArgs {
 // Column of element j of a thread's v-th group of E. Aligned rows: E neighbours
 // (16- or 32-byte accesses); others: one column a lane, so that a warp's access is
 // contiguous.
-template <bool VEC, int E = 8>
+template <bool VEC, int E>
 __device__ __forceinline__ int column(int v, int j, int threads) {
   return VEC ? (v * threads + (int)threadIdx.x) * E + j : (v * E + j) * threads + (int)threadIdx.x;
 }
-
-template <typename T, int E>
-struct alignas(sizeof(T) * E >= 16 ? 16 : sizeof(T) * E) Group {
-  T e[E];
-};
-
-template <typename T, bool VEC, int E = 8>
-__device__ __forceinline__ Group<T, E> load_group(const T* row, int v, int threads, int H) {
-  Group<T, E> p;
+template <typename T, bool VEC, int E>
+__device__ __forceinline__ void load_group(Group<T, E>& p, const T* row, int v, int threads, int H) {
   if constexpr (VEC) {
     const int c = column<true, E>(v, 0, threads);
-    if (c < H) {
-      if constexpr (sizeof(p) >= 16) {
-#pragma unroll
-        for (int i = 0; i < (int)(sizeof(p) / 16); ++i)
-          reinterpret_cast<uint4*>(&p)[i] = reinterpret_cast<const uint4*>(row + c)[i];
-      } else {
-        *reinterpret_cast<uint2*>(&p) = *reinterpret_cast<const uint2*>(row + c);
-      }
-      return p;
-    }
-#pragma unroll
-    for (int j = 0; j < E; ++j) p.e[j] = from_f32<T>(0.f);
+    if (c < H) p.load(row + c);
+    else p.zero();
   } else {
 #pragma unroll
     for (int j = 0; j < E; ++j) {
@@ -86,21 +68,12 @@ __device__ __forceinline__ Group<T, E> load_group(const T* row, int v, int threa
       p.e[j] = c < H ? row[c] : from_f32<T>(0.f);
     }
   }
-  return p;
 }
-template <typename T, bool VEC, int E = 8>
+template <typename T, bool VEC, int E>
 __device__ __forceinline__ void store_group(T* row, const Group<T, E>& p, int v, int threads, int H) {
   if constexpr (VEC) {
     const int c = column<true, E>(v, 0, threads);
-    if (c < H) {
-      if constexpr (sizeof(p) >= 16) {
-#pragma unroll
-        for (int i = 0; i < (int)(sizeof(p) / 16); ++i)
-          reinterpret_cast<uint4*>(row + c)[i] = reinterpret_cast<const uint4*>(&p)[i];
-      } else {
-        *reinterpret_cast<uint2*>(row + c) = *reinterpret_cast<const uint2*>(&p);
-      }
-    }
+    if (c < H) p.store(row + c);
   } else {
 #pragma unroll
     for (int j = 0; j < E; ++j) {
@@ -109,31 +82,83 @@ __device__ __forceinline__ void store_group(T* row, const Group<T, E>& p, int v,
     }
   }
 }
-template <typename T, bool VEC, int E>
-__device__ __forceinline__ void weights_of(float* w, const void* p, int v, int threads, int H) {
-  const Group<T, E> q = load_group<T, VEC, E>(reinterpret_cast<const T*>(p), v, threads, H);
+// A group of factors along the columns: p + one, or `none` throughout without p.
+template <typename W, bool VEC, int E>
+__device__ __forceinline__ void factors(float* w, const void* p, float one, float none, int v, int threads, int H) {
+  if (p) {
+    Group<W, E> q;
+    load_group<W, VEC, E>(q, reinterpret_cast<const W*>(p), v, threads, H);
+    q.unpack(w);
 #pragma unroll
-  for (int j = 0; j < E; ++j) w[j] = to_f32(q.e[j]);
+    for (int j = 0; j < E; ++j) w[j] += one;
+  } else {
+#pragma unroll
+    for (int j = 0; j < E; ++j) w[j] = none;
+  }
 }
-// Sum over the block of NV group sums a thread: a butterfly over the lanes for
-// each group index, then one over the at most 32 warp sums, in index order.
+
+// Sums of four values over the warp, six shuffles: lanes 8 g .. 8 g + 7 get the sum of
+// v[g]. Each sum is taken in the order of warp_sum's butterfly (partners 16, 8, 4, 2,
+// 1 lanes apart), whose bits it has.
+__device__ __forceinline__ float warp_sum4(const float (&v)[4]) {
+  const int lane = threadIdx.x & 31;
+  const bool hi = lane & 16, odd = lane & 8;
+  float a = hi ? v[2] : v[0], b = hi ? v[3] : v[1];
+  a += __shfl_xor_sync(0xffffffffu, hi ? v[0] : v[2], 16);
+  b += __shfl_xor_sync(0xffffffffu, hi ? v[1] : v[3], 16);
+  float s = odd ? b : a;
+  s += __shfl_xor_sync(0xffffffffu, odd ? a : b, 8);
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+
+// Sum over the block of NV group sums a thread (1 or 4): a butterfly over the lanes
+// for each group index, then one over the at most 32 warp sums, in index order.
 // `red`: 32 floats that no other reduction of the same row uses.
 template <int NV>
 __device__ __forceinline__ float row_sum(const float (&s)[NV], float* red) {
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, nw = blockDim.x >> 5;
-#pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    const float t = warp_sum(s[v]);
-    if (lane == 0) red[v * nw + wid] = t;
+  if constexpr (NV == 4) {
+    const float t = warp_sum4(s);
+    if ((lane & 7) == 0) red[(lane >> 3) * nw + wid] = t;
+  } else {
+    const float t = warp_sum(s[0]);
+    if (lane == 0) red[wid] = t;
   }
   __syncthreads();
   return warp_sum(lane < NV * nw ? red[lane] : 0.f);
 }
 
+// u rounded to the residual's type or not, gated, scaled and added: y and the sums of
+// its squares.
+template <typename T, bool VEC, int NV, int NS, bool GATED, bool ROUND>
+__device__ __forceinline__ void add_branch(Group<T, 8> (&x)[NV], const float* u, float grow, const void* gate, float scale,
+                                           int v, int n, int H, float (&s)[NS]) {
+  float f[8], g[8];
+  x[v].unpack(f);
+  if (GATED) factors<T, VEC, 8>(g, gate, 0.f, grow, v, n, H);
+  float b[8];
+  if (ROUND) {
+    Group<T, 8> r;
+    r.pack(u);
+    r.unpack(b);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = u[j];
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] += scale * (GATED ? b[j] * g[j] : b[j]);
+  x[v].pack(f);
+  x[v].unpack(f);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s[NS == 1 ? 0 : v] += f[j] * f[j];
+}
+
 // One row a CTA. NV groups of eight a thread; SEQ: rows above 8192 columns add a
 // thread's groups one after the other, shorter ones sum each group on its own.
-template <typename T, typename W, bool VEC, int NV, bool SEQ>
-__global__ void __launch_bounds__(1024, 1) block_norms_kernel(BlockNormArgs a) {
+template <typename T, typename W, bool VEC, int NV, bool SEQ, bool GATED>
+__global__ void __launch_bounds__(1024, 1) block_norms_kernel(const BlockNormArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   __shared__ float red[2][32];
@@ -144,76 +169,61 @@ __global__ void __launch_bounds__(1024, 1) block_norms_kernel(BlockNormArgs a) {
   const T* dr = reinterpret_cast<const T*>(a.delta) + row * a.ldd;
   Group<T, 8> x[NV], d[NV];
 #pragma unroll
-  for (int v = 0; v < NV; ++v) d[v] = load_group<T, VEC>(dr, v, n, H);
+  for (int v = 0; v < NV; ++v) load_group<T, VEC, 8>(d[v], dr, v, n, H);
 #pragma unroll
-  for (int v = 0; v < NV; ++v) x[v] = load_group<T, VEC>(xr, v, n, H);
+  for (int v = 0; v < NV; ++v) load_group<T, VEC, 8>(x[v], xr, v, n, H);
   const float one = a.offset_one ? 1.f : 0.f;
   float r1 = 1.f;
   if (a.post) {
     float s[NS] = {};
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
+    for (int v = 0; v < NV; ++v) {
+      float f[8];
+      d[v].unpack(f);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float f = to_f32(d[v].e[j]);
-        s[SEQ ? 0 : v] += f * f;
-      }
+      for (int j = 0; j < 8; ++j) s[SEQ ? 0 : v] += f[j] * f[j];
+    }
+#pragma unroll
+    for (int v = 0; v < NV; ++v) d[v].hold();
     r1 = rsqrtf(row_sum(s, red[0]) / (float)H + a.eps);
   }
-  const float grow = a.gate_kind == kGateRow ? to_f32(reinterpret_cast<const T*>(a.gate)[row]) : 1.f;
+  const float grow = GATED && a.gate_kind == kGateRow ? to_f32(reinterpret_cast<const T*>(a.gate)[row]) : 1.f;
+  const void* gate = nullptr;  // a gate along the columns
+  if (GATED && a.gate_kind == kGateChannel) gate = a.gate;
+  if (GATED && a.gate_kind == kGateElement) gate = reinterpret_cast<const T*>(a.gate) + row * a.ldg;
   T* yr = reinterpret_cast<T*>(a.y) + row * a.ldy;
   float s[NS] = {};
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    float w[8], g[8];
-    if (a.post) weights_of<W, VEC, 8>(w, a.post, v, n, H);
-    if (a.gate_kind == kGateChannel) weights_of<T, VEC, 8>(g, a.gate, v, n, H);
-    if (a.gate_kind == kGateElement)
-      weights_of<T, VEC, 8>(g, reinterpret_cast<const T*>(a.gate) + row * a.ldg, v, n, H);
+    float u[8];
+    d[v].unpack(u);
+    if (a.post) {
+      float w[8];
+      factors<W, VEC, 8>(w, a.post, one, 1.f, v, n, H);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float u = to_f32(d[v].e[j]);
-      if (a.post) u = u * r1 * (w[j] + one);
-      if (a.round_branch) u = to_f32(from_f32<T>(u));
-      if (a.gate_kind == kGateRow) u *= grow;
-      else if (a.gate_kind != kGateNone) u *= g[j];
-      x[v].e[j] = from_f32<T>(to_f32(x[v].e[j]) + a.scale * u);
-      const float f = to_f32(x[v].e[j]);
-      s[SEQ ? 0 : v] += f * f;
+      for (int j = 0; j < 8; ++j) u[j] = u[j] * r1 * w[j];
     }
-    store_group<T, VEC>(yr, x[v], v, n, H);
+    if (a.round_branch) add_branch<T, VEC, NV, NS, GATED, true>(x, u, grow, gate, a.scale, v, n, H, s);
+    else add_branch<T, VEC, NV, NS, GATED, false>(x, u, grow, gate, a.scale, v, n, H, s);
+    store_group<T, VEC, 8>(yr, x[v], v, n, H);
   }
   if (threadIdx.x == 0 && a.r1) a.r1[row] = r1;
   if (!a.pre) return;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) x[v].hold();
   const float r2 = rsqrtf(row_sum(s, red[1]) / (float)H + a.eps);
   if (threadIdx.x == 0 && a.r2) a.r2[row] = r2;
   T* hr = reinterpret_cast<T*>(a.h) + row * a.ldh;
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    float w[8];
-    weights_of<W, VEC, 8>(w, a.pre, v, n, H);
+    float f[8], w[8];
+    factors<W, VEC, 8>(w, a.pre, one, 1.f, v, n, H);
+    x[v].unpack(f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[v].e[j] = from_f32<T>(to_f32(x[v].e[j]) * r2 * (w[j] + one));
-    store_group<T, VEC>(hr, x[v], v, n, H);
+    for (int j = 0; j < 8; ++j) f[j] = f[j] * r2 * w[j];
+    x[v].pack(f);
+    store_group<T, VEC, 8>(hr, x[v], v, n, H);
   }
-}
-
-// Three sums over the block in one round: red holds 3 x 32 floats.
-__device__ __forceinline__ void row_sums3(float& a, float& b, float& c, float (*red)[32]) {
-  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  a = warp_sum(a);
-  b = warp_sum(b);
-  c = warp_sum(c);
-  if (lane == 0) {
-    red[0][wid] = a;
-    red[1][wid] = b;
-    red[2][wid] = c;
-  }
-  __syncthreads();
-  const bool in = lane < nw;
-  a = warp_sum(in ? red[0][lane] : 0.f);
-  b = warp_sum(in ? red[1][lane] : 0.f);
-  c = warp_sum(in ? red[2][lane] : 0.f);
 }
 
 // Backward: a CTA walks the rows blockIdx.x, + gridDim.x, ... and keeps its
@@ -222,122 +232,138 @@ __device__ __forceinline__ void row_sums3(float& a, float& b, float& c, float (*
 //
 // Both means come from one round of sums: with c = gate * post * dhat and
 // b = dy + r2 g, mean(w * dhat) = scale * (sum c b - r2 m sum c yhat) / H where
-// m = mean(g * yhat), so neither waits for the other. Groups of four columns leave
-// registers for the next row's loads to be under way while this row's sums are taken.
-constexpr int kBwdE = 4;
-
-template <typename T, bool VEC, int NV>
-struct BwdRow {
-  Group<T, kBwdE> y[NV], d[NV], ty[NV], th[NV];
-  __device__ __forceinline__ void load(const BlockNormArgs& a, int64_t row, int n) {
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      d[v] = load_group<T, VEC, kBwdE>(reinterpret_cast<const T*>(a.delta) + row * a.ldd, v, n, a.H);
-      if (a.dh) {
-        y[v] = load_group<T, VEC, kBwdE>(reinterpret_cast<const T*>(a.y) + row * a.ldy, v, n, a.H);
-        th[v] = load_group<T, VEC, kBwdE>(reinterpret_cast<const T*>(a.dh) + row * a.lddh, v, n, a.H);
-      } else {
-#pragma unroll
-        for (int j = 0; j < kBwdE; ++j) y[v].e[j] = th[v].e[j] = from_f32<T>(0.f);
-      }
-      if (a.dy) {
-        ty[v] = load_group<T, VEC, kBwdE>(reinterpret_cast<const T*>(a.dy) + row * a.lddy, v, n, a.H);
-      } else {
-#pragma unroll
-        for (int j = 0; j < kBwdE; ++j) ty[v].e[j] = from_f32<T>(0.f);
-      }
-    }
-  }
-};
-// Weights as factors: 1 without post, 0 without dh (whose rows are zeros then too).
-template <typename W, bool VEC>
-__device__ __forceinline__ void factors(float* w, const void* p, float one, float none, int v, int n, int H) {
-  if (p) {
-    weights_of<W, VEC, kBwdE>(w, p, v, n, H);
-#pragma unroll
-    for (int j = 0; j < kBwdE; ++j) w[j] += one;
-  } else {
-#pragma unroll
-    for (int j = 0; j < kBwdE; ++j) w[j] = none;
-  }
-}
-
-template <typename T, typename W, bool VEC, int NV, bool GATED>
-__global__ void __launch_bounds__(1024, 1) block_norms_bwd_kernel(const BlockNormArgs a) {
-  constexpr int E = kBwdE;
+// m = mean(g * yhat), so neither waits for the other.
+template <typename T, typename W, bool VEC, int NV, bool GATED, int MAXT>
+__global__ void __launch_bounds__(MAXT, 1024 / MAXT) block_norms_bwd_kernel(const BlockNormArgs a) {
+  constexpr int E = 16 / sizeof(T);  // 16-byte groups
   pdl_launch_dependents();
   pdl_wait();
-  __shared__ float red[2][3][32];
-  const int n = blockDim.x, H = a.H;
+  __shared__ float red[2][4][32];
+  const int n = blockDim.x, H = a.H, lane = threadIdx.x & 31, wid = threadIdx.x >> 5, nw = n >> 5;
   const float one = a.offset_one ? 1.f : 0.f, inv_h = 1.f / (float)H;
   const void* pre = a.dh ? a.pre : nullptr;
   float cpost[NV][E] = {}, cpre[NV][E] = {}, cgate[GATED ? NV : 1][E] = {};
   int flip = 0;
-  BwdRow<T, VEC, NV> in;
-  if ((int64_t)blockIdx.x < a.T) in.load(a, blockIdx.x, n);
   for (int64_t row = blockIdx.x; row < a.T; row += gridDim.x, flip ^= 1) {
     // the sums' buffers alternate between rows: a thread may be writing the next
     // row's while a slower one still reads this row's
+    Group<T, E> y[NV], d[NV], ty[NV], th[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      load_group<T, VEC, E>(d[v], reinterpret_cast<const T*>(a.delta) + row * a.ldd, v, n, H);
+      if (a.dh) {
+        load_group<T, VEC, E>(y[v], reinterpret_cast<const T*>(a.y) + row * a.ldy, v, n, H);
+        load_group<T, VEC, E>(th[v], reinterpret_cast<const T*>(a.dh) + row * a.lddh, v, n, H);
+      } else {
+        y[v].zero();
+        th[v].zero();
+      }
+      if (a.dy) load_group<T, VEC, E>(ty[v], reinterpret_cast<const T*>(a.dy) + row * a.lddy, v, n, H);
+      else ty[v].zero();
+    }
     const float r1 = a.post ? a.r1[row] : 1.f, r2 = a.dh ? a.r2[row] : 0.f;
     const float grow = GATED && a.gate_kind == kGateRow ? to_f32(reinterpret_cast<const T*>(a.gate)[row]) : 1.f;
     const void* gate = nullptr;  // a gate along the columns
     if (GATED && a.gate_kind == kGateChannel) gate = a.gate;
     if (GATED && a.gate_kind == kGateElement) gate = reinterpret_cast<const T*>(a.gate) + row * a.ldg;
-    float s1 = 0.f, s2 = 0.f, s3 = 0.f;
+    float s[4] = {};
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      float wq[E], wp[E], g[E];
-      factors<W, VEC>(wq, pre, one, 0.f, v, n, H);
-      factors<W, VEC>(wp, a.post, one, 1.f, v, n, H);
-      if (GATED) factors<T, VEC>(g, gate, 0.f, 1.f, v, n, H);
+      float c[E], b[E], w[E], f[E];
+      d[v].unpack(c);
+      factors<W, VEC, E>(w, a.post, one, 1.f, v, n, H);
+#pragma unroll
+      for (int j = 0; j < E; ++j) c[j] *= r1 * w[j];
+      if (GATED) {
+        factors<T, VEC, E>(w, gate, 0.f, 1.f, v, n, H);
+#pragma unroll
+        for (int j = 0; j < E; ++j) c[j] *= w[j];
+      }
+      ty[v].unpack(b);
+      factors<W, VEC, E>(w, pre, one, 0.f, v, n, H);
+      float yh[E];
+      y[v].unpack(yh);
+      th[v].unpack(f);
 #pragma unroll
       for (int j = 0; j < E; ++j) {
-        const float yh = to_f32(in.y[v].e[j]) * r2, t = to_f32(in.th[v].e[j]);
-        float c = to_f32(in.d[v].e[j]) * r1 * wp[j];
-        if (GATED) c *= g[j];
-        const float gq = t * wq[j];
-        cpre[v][j] += t * yh;
-        s1 += gq * yh;
-        s2 += c * (to_f32(in.ty[v].e[j]) + r2 * gq);
-        s3 += c * yh;
+        const float t = yh[j] * r2, g = f[j] * w[j];
+        cpre[v][j] += f[j] * t;
+        s[0] += g * t;
+        s[1] += c[j] * (b[j] + r2 * g);
+        s[2] += c[j] * t;
       }
     }
-    BwdRow<T, VEC, NV> cur = in;
-    if (NV <= 2 && row + gridDim.x < a.T) in.load(a, row + gridDim.x, n);
-    row_sums3(s1, s2, s3, red[flip]);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      y[v].hold();
+      d[v].hold();
+      ty[v].hold();
+      th[v].hold();
+    }
+    const float t = warp_sum4(s);
+    if ((lane & 7) == 0) red[flip][lane >> 3][wid] = t;
+    __syncthreads();
+    float q[4];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) q[k] = lane < nw ? red[flip][k][lane] : 0.f;
+    q[3] = 0.f;
+    const float total = warp_sum4(q);
+    const float s1 = __shfl_sync(0xffffffffu, total, 0), s2 = __shfl_sync(0xffffffffu, total, 8),
+                s3 = __shfl_sync(0xffffffffu, total, 16);
     const float m = r2 * s1 * inv_h;              // dt = b - m yhat
     const float along = a.scale * (s2 - m * s3);  // sum of scale * dt * c, without a row gate
     const float m1 = a.post ? along * grow * inv_h : 0.f;
     if (GATED && a.gate_kind == kGateRow && a.dgate && threadIdx.x == 0)
       reinterpret_cast<T*>(a.dgate)[row] = from_f32<T>(along);
+    const float mr2 = m * r2;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      float wq[E], wp[E], g[E];
-      factors<W, VEC>(wq, pre, one, 0.f, v, n, H);
-      factors<W, VEC>(wp, a.post, one, 1.f, v, n, H);
-      if (GATED) factors<T, VEC>(g, gate, 0.f, 1.f, v, n, H);
-      Group<T, E> ox, od, og;
+      float dt[E], w[E], f[E];
+      ty[v].unpack(dt);
+      factors<W, VEC, E>(w, pre, one, 0.f, v, n, H);
+      th[v].unpack(f);
+#pragma unroll
+      for (int j = 0; j < E; ++j) dt[j] += r2 * (f[j] * w[j]);
+      y[v].unpack(f);
+#pragma unroll
+      for (int j = 0; j < E; ++j) dt[j] -= f[j] * mr2;
+      if (a.dx) {
+        ty[v].pack(dt);
+        store_group<T, VEC, E>(reinterpret_cast<T*>(a.dx) + row * a.ldo, ty[v], v, n, H);
+      }
+      factors<W, VEC, E>(w, a.post, one, 1.f, v, n, H);
+      d[v].unpack(f);
 #pragma unroll
       for (int j = 0; j < E; ++j) {
-        const float dt = to_f32(cur.ty[v].e[j]) + r2 * (to_f32(cur.th[v].e[j]) * wq[j]) - to_f32(cur.y[v].e[j]) * r2 * m;
-        const float dhat = to_f32(cur.d[v].e[j]) * r1;
-        float du = a.scale * dt;
-        if (GATED) {
-          const float dg = du * dhat * wp[j];
-          cgate[v][j] += dg;
-          og.e[j] = from_f32<T>(dg);
-          du *= g[j] * grow;
-        }
-        cpost[v][j] += du * dhat;
-        ox.e[j] = from_f32<T>(dt);
-        od.e[j] = from_f32<T>(r1 * (du * wp[j] - dhat * m1));
+        f[j] *= r1;  // dhat
+        dt[j] *= a.scale;
       }
-      if (a.dx) store_group<T, VEC, E>(reinterpret_cast<T*>(a.dx) + row * a.ldo, ox, v, n, H);
-      if (a.ddelta) store_group<T, VEC, E>(reinterpret_cast<T*>(a.ddelta) + row * a.ldo, od, v, n, H);
-      if (GATED && a.gate_kind == kGateElement && a.dgate)
-        store_group<T, VEC, E>(reinterpret_cast<T*>(a.dgate) + row * a.ldo, og, v, n, H);
+      if (GATED) {
+        float g[E];
+        factors<T, VEC, E>(g, gate, 0.f, grow, v, n, H);
+        float dg[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          dg[j] = dt[j] * f[j] * w[j];
+          cgate[v][j] += dg[j];
+          dt[j] *= g[j];
+        }
+        if (a.gate_kind == kGateElement && a.dgate) {
+          Group<T, E> o;
+          o.pack(dg);
+          store_group<T, VEC, E>(reinterpret_cast<T*>(a.dgate) + row * a.ldo, o, v, n, H);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        cpost[v][j] += dt[j] * f[j];
+        dt[j] = r1 * (dt[j] * w[j] - f[j] * m1);
+      }
+      if (a.ddelta) {
+        d[v].pack(dt);
+        store_group<T, VEC, E>(reinterpret_cast<T*>(a.ddelta) + row * a.ldo, d[v], v, n, H);
+      }
     }
-    if (NV > 2 && row + gridDim.x < a.T) in.load(a, row + gridDim.x, n);
   }
   float* part = a.part;
   auto put = [&](const float (&c)[E], int v) {
@@ -401,37 +427,44 @@ static inline int round32(int v) { return (v + 31) / 32 * 32; }
 // (8192 x 4096 bf16: see kFewRows); both add in the same order. Unaligned rows are
 // dealt to the lanes by the thread count, so there the choice goes by the width alone.
 constexpr int kFewRows = 4;  // rows an SM
-template <typename T, typename W, bool VEC>
-static int launch_fwd(const BlockNormArgs& a, int num_sms, cudaStream_t st) {
+template <typename T, typename W, bool VEC, bool GATED>
+static int launch_fwd_gate(const BlockNormArgs& a, int num_sms, cudaStream_t st) {
   const int groups = (a.H + 7) / 8;
   const dim3 grid((unsigned)a.T);
   cudaError_t e;
   if (groups > 1024)
-    e = launch_k(block_norms_kernel<T, W, VEC, 4, true>, grid, dim3(1024), 0, st, 1, a);
+    e = launch_k(block_norms_kernel<T, W, VEC, 4, true, GATED>, grid, dim3(1024), 0, st, 1, a);
   else if (VEC && a.T <= (int64_t)kFewRows * num_sms)
-    e = launch_k(block_norms_kernel<T, W, VEC, 1, false>, grid, dim3(round32(groups)), 0, st, 1, a);
+    e = launch_k(block_norms_kernel<T, W, VEC, 1, false, GATED>, grid, dim3(round32(groups)), 0, st, 1, a);
   else
-    e = launch_k(block_norms_kernel<T, W, VEC, 4, false>, grid, dim3(round32((groups + 3) / 4)), 0, st, 1, a);
+    e = launch_k(block_norms_kernel<T, W, VEC, 4, false, GATED>, grid, dim3(round32((groups + 3) / 4)), 0, st, 1, a);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
-
-static inline int bwd_groups(int H) { return (H + kBwdE - 1) / kBwdE; }
-static inline int bwd_threads(int H) {
-  const int g = bwd_groups(H);
-  return round32(g < 1024 ? g : 1024);
+template <typename T, typename W, bool VEC>
+static int launch_fwd(const BlockNormArgs& a, int num_sms, cudaStream_t st) {
+  return a.gate_kind == kGateNone ? launch_fwd_gate<T, W, VEC, false>(a, num_sms, st)
+                                  : launch_fwd_gate<T, W, VEC, true>(a, num_sms, st);
 }
 
+// Backward: a 16-byte group a thread up to 1024 threads, more groups for wider rows.
+// Rows of at most 512 groups leave room for several CTAs on an SM, one's loads under
+// another's sums.
+static inline int bwd_threads(int H, int type) {
+  const int g = type == kElemF32 ? (H + 3) / 4 : (H + 7) / 8;
+  return round32(g < 1024 ? g : 1024);
+}
 template <typename T, typename W, bool VEC, bool GATED>
 static int launch_bwd_gate(const BlockNormArgs& a, int grid, cudaStream_t st) {
-  const int groups = bwd_groups(a.H);
-  const dim3 threads(bwd_threads(a.H));
+  constexpr int E = 16 / sizeof(T), kWide = 32 / E;  // kWide x 1024 groups cover the widest row
+  const int groups = (a.H + E - 1) / E;
+  const dim3 threads(round32(groups < 1024 ? groups : 1024));
   cudaError_t e;
-  if (groups > 2048)
-    e = launch_k(block_norms_bwd_kernel<T, W, VEC, 8, GATED>, dim3(grid), threads, 0, st, 1, a);
-  else if (groups > 1024)
-    e = launch_k(block_norms_bwd_kernel<T, W, VEC, 2, GATED>, dim3(grid), threads, 0, st, 1, a);
+  if (groups > 1024)
+    e = launch_k(block_norms_bwd_kernel<T, W, VEC, kWide, GATED, 1024>, dim3(grid), threads, 0, st, 1, a);
+  else if (groups > 512)
+    e = launch_k(block_norms_bwd_kernel<T, W, VEC, 1, GATED, 1024>, dim3(grid), threads, 0, st, 1, a);
   else
-    e = launch_k(block_norms_bwd_kernel<T, W, VEC, 1, GATED>, dim3(grid), threads, 0, st, 1, a);
+    e = launch_k(block_norms_bwd_kernel<T, W, VEC, 1, GATED, 512>, dim3(grid), threads, 0, st, 1, a);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 template <typename T, typename W, bool VEC>
@@ -460,8 +493,8 @@ int b200_block_norms_max_width() { return 4 * 1024 * 8; }
 
 // CTAs of the backward pass (rows of its partial sums) for T rows of H columns: what
 // fits on the SMs at 64 registers a thread.
-int b200_block_norms_bwd_grid(int64_t T, int H, int num_sms) {
-  int per_sm = 1024 / bwd_threads(H);
+int b200_block_norms_bwd_grid(int64_t T, int H, int type, int num_sms) {
+  int per_sm = 1024 / bwd_threads(H, type);
   per_sm = per_sm > 16 ? 16 : per_sm < 1 ? 1 : per_sm;
   const int64_t most = (int64_t)per_sm * num_sms;
   return (int)(T < most ? T : most);
@@ -555,7 +588,7 @@ int b200_block_norms_bwd(const void* y, int64_t ldy, const void* delta, int64_t 
                    rows16(dx, 0) && rows16(ddelta, 0) && rows16(post, 0) && rows16(pre, 0) &&
                    (gate_kind == kGateRow ||
                     (rows16(gate, gate_kind == kGateElement ? ldg : 0) && (gate_kind != kGateElement || rows16(dgate, 0))));
-  const int grid = b200_block_norms_bwd_grid(T, H, num_sms);
+  const int grid = b200_block_norms_bwd_grid(T, H, type, num_sms);
   const int e = by_type(type, w_type, vec, [&](auto t, auto w, auto v) {
     return launch_bwd<decltype(t), decltype(w), decltype(v)::value>(a, grid, st);
   });

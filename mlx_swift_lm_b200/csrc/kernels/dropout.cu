@@ -12,6 +12,7 @@
 // wide multiplications, 2.5 an element here.
 #include "b200_elem.cuh"
 #include "b200_philox.cuh"
+#include "b200_train.h"
 
 namespace b200 {
 
@@ -30,23 +31,20 @@ struct DropoutArgs {
   float scale;
 };
 
-// Bit j: element j of the unit stays.
-__device__ __forceinline__ unsigned keep_bits(const DropoutArgs& a, unsigned row, unsigned unit, uint64_t offset) {
-  uint32_t c[4] = {unit, row, (uint32_t)offset, (uint32_t)(offset >> 32)};
+// The unit's random words. Element 2 w is the low half of word w, 2 w + 1 the high.
+__device__ __forceinline__ void draw(uint32_t (&c)[4], const DropoutArgs& a, unsigned row, unsigned unit, uint64_t offset) {
+  c[0] = unit;
+  c[1] = row;
+  c[2] = (uint32_t)offset;
+  c[3] = (uint32_t)(offset >> 32);
   philox_4x32_10(c, a.seed);
-  unsigned bits = 0;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    bits |= ((c[w] & 0xFFFFu) >= a.cut ? 1u : 0u) << (2 * w);
-    bits |= ((c[w] >> 16) >= a.cut ? 1u : 0u) << (2 * w + 1);
-  }
-  return bits;
 }
 
-// Aligned rows: a thread owns two units at a time (16-byte loads and stores, both
-// under way before the first is drawn).
-constexpr int kUnits = 2;
-template <typename T>
+// Aligned rows: a thread owns a unit at a time, 16-byte loads and stores. Bound by the
+// integer and select instructions of the draw (about 100 for eight elements) at
+// 16-bit types, by memory at fp32. `cut` is compared in the upper half of a word, so
+// that the high halves need no shift.
+template <typename T, bool RES>
 __global__ void __launch_bounds__(256) dropout_vec_kernel(const DropoutArgs a) {
   pdl_launch_dependents();
   pdl_wait();
@@ -54,65 +52,73 @@ __global__ void __launch_bounds__(256) dropout_vec_kernel(const DropoutArgs a) {
   const T* x = reinterpret_cast<const T*>(a.x);
   const T* res = reinterpret_cast<const T*>(a.residual);
   T* y = reinterpret_cast<T*>(a.y);
-  for (unsigned u0 = blockIdx.x * (256u * kUnits) + threadIdx.x; u0 < a.units; u0 += gridDim.x * (256u * kUnits)) {
-    Pack8<T> v[kUnits], q[kUnits];
-    unsigned row[kUnits], unit[kUnits];
+  const uint32_t cut = a.cut << 16;
+  for (unsigned u = blockIdx.x * 256u + threadIdx.x; u < a.units; u += gridDim.x * 256u) {
+    const unsigned row = (unsigned)(((uint64_t)u * a.div_mul) >> a.div_shift);
+    const unsigned unit = u - row * a.units_per_row;
+    const int64_t r = row, c = (int64_t)unit * 8;
+    Group<T, 8> v, q;
+    v.load(x + r * a.ldx + c);
+    if (RES) q.load(res + r * a.ldr + c);
+    uint32_t w[4];
+    draw(w, a, a.row0 + row, unit, offset);
+    float f[8], g[8];
+    v.unpack(f);
+    if (RES) q.unpack(g);
 #pragma unroll
-    for (int i = 0; i < kUnits; ++i) {
-      const unsigned u = u0 + 256u * i;
-      row[i] = (unsigned)(((uint64_t)u * a.div_mul) >> a.div_shift);
-      unit[i] = u - row[i] * a.units_per_row;
-      if (u < a.units) {
-        v[i] = load_pack(x + (int64_t)row[i] * a.ldx + (int64_t)unit[i] * 8);
-        if (res) q[i] = load_pack(res + (int64_t)row[i] * a.ldr + (int64_t)unit[i] * 8);
-      }
+    for (int j = 0; j < 4; ++j) {
+      f[2 * j] = (w[j] << 16) >= cut ? f[2 * j] * a.scale : 0.f;
+      f[2 * j + 1] = w[j] >= cut ? f[2 * j + 1] * a.scale : 0.f;
     }
+    if (RES) {
 #pragma unroll
-    for (int i = 0; i < kUnits; ++i) {
-      const unsigned bits = keep_bits(a, a.row0 + row[i], unit[i], offset);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float f = (bits >> j) & 1u ? to_f32(v[i].e[j]) * a.scale : 0.f;
-        if (res) f += to_f32(q[i].e[j]);
-        v[i].e[j] = from_f32<T>(f);
-      }
-      if (u0 + 256u * i < a.units) store_pack(y + (int64_t)row[i] * a.ldy + (int64_t)unit[i] * 8, v[i]);
+      for (int j = 0; j < 8; ++j) f[j] += g[j];
     }
+    v.pack(f);
+    v.store(y + r * a.ldy + c);
   }
 }
 
 // Rows of any width, stride and alignment: a warp owns 256 columns. Each lane
 // draws one unit's bits; the elements then go by column = lane + 32 j, so that
 // every access of the warp is contiguous, with the bits fetched from their lane.
-template <typename T>
+template <typename T, bool RES>
 __global__ void __launch_bounds__(256) dropout_any_kernel(const DropoutArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   const uint64_t offset = a.offset + (a.offset_ptr ? (uint64_t)*a.offset_ptr : 0ull);
   const int lane = threadIdx.x & 31;
-  const T* x = reinterpret_cast<const T*>(a.x);
-  const T* res = reinterpret_cast<const T*>(a.residual);
-  T* y = reinterpret_cast<T*>(a.y);
+  const uint32_t cut = a.cut << 16;
   // here a "unit" of the division is a warp's chunk of 256 columns
   for (unsigned u = blockIdx.x * 8u + (threadIdx.x >> 5); u < a.units; u += gridDim.x * 8u) {
     const unsigned row = (unsigned)(((uint64_t)u * a.div_mul) >> a.div_shift);
     const unsigned chunk = u - row * a.units_per_row;
     const int64_t r = row;
-    const int c0 = (int)(chunk * 256u);
-    float v[8], q[8];
+    const int c0 = (int)(chunk * 256u) + lane;
+    const T* x = reinterpret_cast<const T*>(a.x) + r * a.ldx + c0;
+    const T* res = reinterpret_cast<const T*>(a.residual) + r * a.ldr + c0;
+    T* y = reinterpret_cast<T*>(a.y) + r * a.ldy + c0;
+    T v[8], q[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c0 + 32 * j < a.K) {
+        v[j] = x[32 * j];
+        if (RES) q[j] = res[32 * j];
+      }
+    uint32_t w[4];
+    draw(w, a, a.row0 + row, chunk * 32u + lane, offset);
+    unsigned bits = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) bits |= ((w[j] << 16) >= cut ? 1u << (2 * j) : 0u) | (w[j] >= cut ? 2u << (2 * j) : 0u);
+    const unsigned mine = 1u << (lane & 7);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int c = c0 + 32 * j + lane;
-      v[j] = c < a.K ? to_f32(x[r * a.ldx + c]) : 0.f;
-      q[j] = res && c < a.K ? to_f32(res[r * a.ldr + c]) : 0.f;
-    }
-    const unsigned bits = keep_bits(a, a.row0 + row, chunk * 32u + lane, offset);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = c0 + 32 * j + lane;
       const unsigned b = __shfl_sync(0xffffffffu, bits, 4 * j + (lane >> 3));
-      const float f = ((b >> (lane & 7)) & 1u ? v[j] * a.scale : 0.f) + q[j];
-      if (c < a.K) y[r * a.ldy + c] = from_f32<T>(f);
+      if (c0 + 32 * j < a.K) {
+        float f = b & mine ? to_f32(v[j]) * a.scale : 0.f;
+        if (RES) f += to_f32(q[j]);
+        y[32 * j] = from_f32<T>(f);
+      }
     }
   }
 }
@@ -142,12 +148,13 @@ static int launch_dropout(DropoutArgs a, int64_t rows, bool vec, int num_sms, cu
     a.y = y + r0 * a.ldy * (int64_t)sizeof(T);
     a.row0 = (unsigned)r0;
     a.units = (unsigned)(n * upr);
-    const unsigned per = vec ? 256 * kUnits : 8;
+    const unsigned per = vec ? 256 : 8;
     unsigned grid = (a.units + per - 1) / per;
     const unsigned most = (unsigned)num_sms * 8;  // no more CTAs than can be resident
     grid = grid < most ? grid : most;
-    cudaError_t e = vec ? launch_k(dropout_vec_kernel<T>, dim3(grid), dim3(256), 0, st, 1, a)
-                        : launch_k(dropout_any_kernel<T>, dim3(grid), dim3(256), 0, st, 1, a);
+    void (*kernel)(const DropoutArgs) = vec ? (a.residual ? dropout_vec_kernel<T, true> : dropout_vec_kernel<T, false>)
+                                            : (a.residual ? dropout_any_kernel<T, true> : dropout_any_kernel<T, false>);
+    const cudaError_t e = launch_k(kernel, dim3(grid), dim3(256), 0, st, 1, a);
     if (e != cudaSuccess) return (int)e;
   }
   return (int)cudaGetLastError();
@@ -160,12 +167,12 @@ using namespace b200;
 extern "C" {
 
 // y[rows, K] = dropout(x) (+ residual); strides in elements, type: ElemType of all
-// three. 0 <= cut <= 65536 (scale is the caller's, 0 where cut is 65536).
+// three. 0 <= cut < 65536 (a call that drops everything needs no kernel).
 // Returns 0, a CUDA error code, or -1 for arguments out of range.
 int b200_dropout(const void* x, int64_t ldx, const void* residual, int64_t ldr, void* y, int64_t ldy, int64_t rows,
                  int K, int type, uint64_t seed, uint64_t offset, const int64_t* offset_ptr, int cut, float scale,
                  int num_sms, cudaStream_t st) {
-  if (rows < 0 || K < 0 || rows > 0xFFFFFFFFll || cut < 0 || cut > 65536 || type < 0 || type > 2) return -1;
+  if (rows < 0 || K < 0 || rows > 0xFFFFFFFFll || cut < 0 || cut > 65535 || type < 0 || type > 2) return -1;
   if (rows == 0 || K == 0) return 0;
   DropoutArgs a = {};
   a.x = x;

@@ -29,6 +29,7 @@
 // arithmetic and the stores run under the next tile's product. Tiles leave through
 // shared memory by TMA; the fp32 sums of dh are added up in L2 by its reduction.
 #include "b200_common.cuh"
+#include "b200_train.h"
 
 namespace b200 {
 

@@ -151,17 +151,6 @@ def stream_ptr(device=None) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
-def launch(fn, device: torch.device, *args) -> int:
-    """Call a kernel entry point with torch's current stream of `device` as its
-    last argument, with that device current (a launch goes to the calling
-    thread's device, whatever its stream)."""
-    st = torch._C._cuda_getCurrentRawStream(device.index)
-    if device.index == torch.cuda.current_device():
-        return fn(*args, st)
-    with torch.cuda.device(device):
-        return fn(*args, st)
-
-
 def check(rc: int, what: str):
     if rc != 0:
         raise KernelError(f"{what} failed with code {rc}")

@@ -2,24 +2,9 @@
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from . import _lib
+from . import _autograd, _lib
 from . import reference as ref
-from ._args import ELEM, elem_code, rows2d, same_device
-from .linear import num_sms
-
-_lib.register_signatures({
-    "b200_block_norms": (_lib.i32, [_lib.vp, _lib.i64, _lib.vp, _lib.i64, _lib.vp, _lib.vp, _lib.i32, _lib.vp, _lib.i64,
-                                    _lib.i32, _lib.vp, _lib.i64, _lib.vp, _lib.i64, _lib.vp, _lib.vp, _lib.i64,
-                                    _lib.i32, _lib.i32, _lib.f32, _lib.f32, _lib.i32, _lib.i32, _lib.i32, _lib.vp]),
-    "b200_block_norms_bwd": (_lib.i32, [_lib.vp, _lib.i64, _lib.vp, _lib.i64, _lib.vp, _lib.vp, _lib.i32, _lib.vp,
-                                        _lib.i64, _lib.i32, _lib.vp, _lib.vp, _lib.vp, _lib.i64, _lib.vp, _lib.i64,
-                                        _lib.vp, _lib.vp, _lib.vp, _lib.vp, _lib.vp, _lib.vp, _lib.i64, _lib.i32,
-                                        _lib.i32, _lib.f32, _lib.i32, _lib.i32, _lib.vp]),
-    "b200_block_norms_max_width": (_lib.i32, []),
-    "b200_block_norms_bwd_grid": (_lib.i32, [_lib.i64, _lib.i32, _lib.i32]),
-}, status_tags=("block_norms",))
 
 
 def add_rmsnorm(x: torch.Tensor, delta: torch.Tensor | None, w: torch.Tensor, eps: float,
@@ -72,101 +57,6 @@ def rmsnorm(x, w, eps, offset_one=False):
     return add_rmsnorm(x, None, w, eps, offset_one=offset_one)
 
 
-_GATE_NONE, _GATE_CHANNEL, _GATE_ROW, _GATE_ELEMENT = range(4)
-
-
-def _gate_kind(gate, x) -> int:
-    if gate is None:
-        return _GATE_NONE
-    if gate.shape == x.shape[-1:]:
-        return _GATE_CHANNEL
-    if gate.shape == x.shape[:-1] + (1,):
-        return _GATE_ROW
-    if gate.shape == x.shape:
-        return _GATE_ELEMENT
-    raise ValueError(f"block_norms: gate {tuple(gate.shape)} is neither {tuple(x.shape[-1:])}, "
-                     f"{tuple(x.shape[:-1]) + (1,)} nor {tuple(x.shape)}")
-
-
-def _block_norms_fwd(x, delta, post_w, pre_w, gate, kind, eps, scale, offset_one, round_branch, y, save):
-    """(y, h, r1, r2); y is written in place when given. r1 / r2 (fp32 [T], the
-    reciprocal RMS of delta and y) are kept for the backward pass with `save`."""
-    H = x.shape[-1]
-    dev = x.device
-    if y is None:
-        y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    h = None if pre_w is None else torch.empty_like(x, memory_format=torch.contiguous_format)
-    x2, d2, y2 = rows2d(x, H), rows2d(delta, H), rows2d(y, H)
-    T = x2.shape[0]
-    r1 = torch.empty(T, dtype=torch.float32, device=dev) if save and post_w is not None else None
-    r2 = torch.empty(T, dtype=torch.float32, device=dev) if save and pre_w is not None else None
-    post_w, pre_w = (None if w is None else w.contiguous() for w in (post_w, pre_w))
-    g = None if gate is None else rows2d(gate, H) if kind == _GATE_ELEMENT else gate.contiguous()
-    w = post_w if post_w is not None else pre_w
-    if T:
-        rc = _lib.launch(
-            _lib.lib().b200_block_norms, dev, x2.data_ptr(), x2.stride(0), d2.data_ptr(), d2.stride(0),
-            _lib.ptr(post_w), _lib.ptr(pre_w), ELEM[x.dtype if w is None else w.dtype], _lib.ptr(g),
-            g.stride(0) if kind == _GATE_ELEMENT else 0, kind, y2.data_ptr(), y2.stride(0), _lib.ptr(h), H,
-            _lib.ptr(r1), _lib.ptr(r2), T, H, ELEM[x.dtype], float(eps), float(scale), 1 if offset_one else 0,
-            1 if round_branch else 0, num_sms(dev))
-        _lib.check(rc, "block_norms")
-        _lib.count(1)
-    return y, h, r1, r2
-
-
-class _BlockNorms(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, delta, post_w, pre_w, gate, kind, eps, scale, offset_one, round_branch):
-        ctx.set_materialize_grads(False)
-        y, h, r1, r2 = _block_norms_fwd(x, delta, post_w, pre_w, gate, kind, eps, scale, offset_one, round_branch,
-                                        None, True)
-        ctx.save_for_backward(y, delta, post_w, pre_w, gate, r1, r2)
-        ctx.kind, ctx.scale, ctx.offset_one = kind, float(scale), bool(offset_one)
-        return y, h
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dh=None):
-        y, delta, post_w, pre_w, gate, r1, r2 = ctx.saved_tensors
-        need_x, need_d, need_post, need_pre, need_gate = ctx.needs_input_grad[:5]
-        none = (None,) * 5
-        if dy is None and dh is None:
-            return (None,) * 5 + none
-        dev, H, kind = y.device, y.shape[-1], ctx.kind
-
-        def like(t, need):
-            return torch.empty_like(t, memory_format=torch.contiguous_format) if need else None
-
-        y2, d2 = rows2d(y, H), rows2d(delta, H)
-        T = y2.shape[0]
-        dx, dd, dgate, dpost, dpre = (like(y, need_x), like(delta, need_d), like(gate, need_gate),
-                                      like(post_w, need_post), like(pre_w, need_pre and dh is not None))
-        if T == 0:
-            for t in (dgate, dpost, dpre):
-                if t is not None:
-                    t.zero_()
-            return (dx, dd, dpost, dpre, dgate) + none
-        dy2 = None if dy is None else rows2d(dy, H)
-        dh2 = None if dh is None else rows2d(dh, H)
-        pw, qw = (None if w is None else w.contiguous() for w in (post_w, pre_w))
-        g = None if gate is None else rows2d(gate, H) if kind == _GATE_ELEMENT else gate.contiguous()
-        w = pw if pw is not None else qw
-        n_part = sum(t is not None for t in (dpost, dpre, dgate if kind == _GATE_CHANNEL else None))
-        L, sms = _lib.lib(), num_sms(dev)
-        part = (torch.empty(n_part * L.b200_block_norms_bwd_grid(T, H, sms) * H, dtype=torch.float32, device=dev)
-                if n_part else None)
-        rc = _lib.launch(
-            L.b200_block_norms_bwd, dev, y2.data_ptr(), y2.stride(0), d2.data_ptr(), d2.stride(0), _lib.ptr(pw),
-            _lib.ptr(qw), ELEM[y.dtype if w is None else w.dtype], _lib.ptr(g), g.stride(0) if kind == _GATE_ELEMENT else 0,
-            kind, _lib.ptr(r1), _lib.ptr(r2), _lib.ptr(dy2), 0 if dy2 is None else dy2.stride(0), _lib.ptr(dh2),
-            0 if dh2 is None else dh2.stride(0), _lib.ptr(dx), _lib.ptr(dd), _lib.ptr(dgate), _lib.ptr(dpost),
-            _lib.ptr(dpre), _lib.ptr(part), T, H, ELEM[y.dtype], ctx.scale, 1 if ctx.offset_one else 0, sms)
-        _lib.check(rc, "block_norms backward")
-        _lib.count(2 if n_part else 1)
-        return (dx, dd, dpost, dpre, dgate) + none
-
-
 def block_norms(x: torch.Tensor, delta: torch.Tensor, post_w: torch.Tensor | None = None,
                 pre_w: torch.Tensor | None = None, eps: float = 1e-6, gate: torch.Tensor | None = None,
                 scale: float = 1.0, offset_one: bool = False, round_branch: bool = False, inplace: bool = False):
@@ -184,39 +74,13 @@ def block_norms(x: torch.Tensor, delta: torch.Tensor, post_w: torch.Tensor | Non
     ``add_rmsnorm(x, rmsnorm(delta, post_w), pre_w)``). `inplace`: y is written
     into x (no gradients).
     """
-    H = x.shape[-1] if x.dim() else 0
-    if x.dim() == 0 or H == 0:
-        raise ValueError("block_norms: x needs at least one column")
-    elem_code(x, "block_norms")
-    if delta.shape != x.shape or delta.dtype != x.dtype:
-        raise ValueError(f"block_norms: delta {tuple(delta.shape)} {delta.dtype} for x {tuple(x.shape)} {x.dtype}")
-    kind = _gate_kind(gate, x)
-    if gate is not None and gate.dtype != x.dtype:
-        raise TypeError(f"block_norms: gate {gate.dtype} for x {x.dtype}")
-    for w in (post_w, pre_w):
-        if w is not None and w.shape != (H,):
-            raise ValueError(f"block_norms: weight {tuple(w.shape)} for rows of {H}")
-        if w is not None and w.dtype != x.dtype and w.dtype != torch.float32:
-            raise TypeError(f"block_norms: weight {w.dtype} for x {x.dtype}")
-    if post_w is not None and pre_w is not None and post_w.dtype != pre_w.dtype:
-        raise TypeError(f"block_norms: post_w {post_w.dtype}, pre_w {pre_w.dtype}")
-    same_device("block_norms", x, delta, post_w, pre_w, gate)
-    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, delta, post_w, pre_w, gate))
-    if inplace:
-        if grad:
-            raise ValueError("block_norms: inplace takes no gradients")
-        rows = x.view(-1, H)
-        if x.numel() and ((H > 1 and rows.stride(1) != 1) or (rows.shape[0] > 1 and rows.stride(0) < H)):
-            raise ValueError("block_norms: inplace needs rows of neighbouring columns that do not overlap")
-    if not x.is_cuda:
+    out = _autograd.for_device(x).block_norms(x, delta, post_w, pre_w, eps, gate, scale, offset_one, round_branch,
+                                              inplace)
+    if out is None:
         y, h = ref.block_norms_ref(x, delta, post_w, pre_w, eps, gate, scale, offset_one, round_branch)
         return (x.copy_(y) if inplace else y), h
-    if H > _lib.lib().b200_block_norms_max_width():
-        raise ValueError(f"block_norms: {H} columns, at most {_lib.lib().b200_block_norms_max_width()}")
-    if grad:
-        return _BlockNorms.apply(x, delta, post_w, pre_w, gate, kind, eps, scale, offset_one, round_branch)
-    return _block_norms_fwd(x, delta, post_w, pre_w, gate, kind, eps, scale, offset_one, round_branch,
-                            x if inplace else None, False)[:2]
+    _lib.count(1)
+    return out
 
 
 def qk_norm_rope_kv(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor | None, cos_sin: torch.Tensor,
