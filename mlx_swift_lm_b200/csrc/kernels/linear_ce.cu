@@ -152,23 +152,30 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // Parts of dh's contraction of `kb` blocks of 64 over `tiles` output tiles: the
-// fewest that (nearly) minimise the rounds of the pairs times their length, so that
-// few rows still fill the machine and the last round is not half empty. A part costs
+// fewest that minimise the rounds of the CTA pairs times their length, so that few
+// rows still fill the machine and the last round is not half empty. A part costs
 // about kPartBlocks blocks beyond its product (its tile's way out). Chosen on the
-// device, where the number of scored rows is known.
-constexpr int kPartBlocks = 6;
-__host__ __device__ inline int choose_parts(int tiles, int kb, int pairs, int most) {
-  int best = 1;
-  int64_t cost = INT64_MAX;
-  for (int s = 1; s <= most && (s == 1 || kb / s >= 16); ++s) {
-    const int64_t rounds = ((int64_t)tiles * s + pairs - 1) / pairs;
-    const int64_t c = rounds * ((kb + s - 1) / s + kPartBlocks);
-    if (c < cost) {
-      cost = c;
-      best = s;
+// device, where the number of scored rows is known, by a whole warp: a lane weighs
+// two of the at most kMostParts choices.
+constexpr int kPartBlocks = 6, kMostParts = 64;
+__device__ __forceinline__ int choose_parts(int tiles, int kb, int pairs, int most) {
+  unsigned best = 0xFFFFFFFFu;
+#pragma unroll
+  for (int i = 0; i < kMostParts / 32; ++i) {
+    const int s = (threadIdx.x & 31) + 32 * i + 1;
+    if (s <= most && (s == 1 || kb >= 16 * s)) {
+      const float rounds = ceilf((float)tiles * (float)s / (float)pairs);
+      const float cost = rounds * (float)((kb + s - 1) / s + kPartBlocks);
+      best = min(best, (unsigned)fminf(cost, 6e7f) * kMostParts + (unsigned)(s - 1));  // the fewer win a tie
     }
   }
-  return best;
+  return (int)(__reduce_min_sync(0xffffffffu, best) % kMostParts) + 1;
+}
+
+// 1 - 2 / (1 + e^2x): off by at most 2^-22 of one, which is enough where the result is
+// rounded to bf16 (the losses take tanhf); 5 instructions for about 20.
+__device__ __forceinline__ float tanh_fast(float x) {
+  return 1.f - __fdividef(2.f, 1.f + ex2(2.f * kLog2e * x));
 }
 
 // The tile walk of one launch: `mt` x `nt` tiles (times `splits` of the
@@ -426,7 +433,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 for (int e = 0; e < 2; ++e) {
                   float z = __uint_as_float(v[j + e]), slope = dl;
                   if (a.cap > 0.f) {
-                    const float q = tanhf(z * a.inv_cap);
+                    const float q = tanh_fast(z * a.inv_cap);
                     z = a.cap * q;
                     slope *= 1.f - q * q;
                   }
@@ -753,7 +760,7 @@ int64_t b200_lce_forward_bytes(int T, int V) { return (int64_t)T * tiles_of(V, k
 // of all CTA pairs, at most 155 MB, and always one.
 static int most_parts(int T, int K, int num_sms) {
   const int64_t s = 8 * (num_sms / 2) / (tiles_of(T, kTileM) * tiles_of(K, kTileN));
-  return (int)(s > 64 ? 64 : s < 1 ? 1 : s);
+  return (int)(s > kMostParts ? kMostParts : s < 1 ? 1 : s);
 }
 // Rows and row stride (elements) of one part of dh's sums.
 static int acc_rows(int T) { return (int)(tiles_of(T, kRowsM) * kRowsM); }

@@ -517,10 +517,13 @@ class DecoderLM:
         delta = None
         attn = torch.empty((T, self.H, self.D), dtype=x.dtype, device=x.device)
         hook = self._after_layer
+        post = None  # the norm delta still has to pass before it is added (sandwich- and post-norm blocks)
         for li, L in enumerate(self.layers):
             if hook is not None and li > 0:
-                x, delta = hook(li - 1, x, delta)
-            h = self._norm(x, delta, L.ln1, L.ln1_b)
+                x, delta = hook(li - 1, x, self._post_norm(delta, post))
+                post = None
+            h = self._norm(x, delta, L.ln1, L.ln1_b, post)
+            post = None
             if L.block == "ffn":  # FFN-only layer (NemotronH "-" / "E")
                 delta = self._mlp(L, h)
                 continue
@@ -532,14 +535,13 @@ class DecoderLM:
                 delta = self._gdn(L, h, fb, kv, li)
             else:
                 delta = self._attention(L, h, fb, kv, li, attn)
-            if L.post_attn_norm is not None:
-                delta = ops.rmsnorm(delta, L.post_attn_norm, cfg.rms_norm_eps, cfg.norm_offset_one)
+            post = L.post_attn_norm
             if L.block == "mixer":
                 continue
-            h = self._norm(x, delta, L.ln2, L.ln2_b)
+            h = self._norm(x, delta, L.ln2, L.ln2_b, post)
             delta = self._mlp(L, h)
-            if L.post_ffn_norm is not None:
-                delta = ops.rmsnorm(delta, L.post_ffn_norm, cfg.rms_norm_eps, cfg.norm_offset_one)
+            post = L.post_ffn_norm
+        delta = self._post_norm(delta, post)
         return self._head(x, delta, fb, return_hidden, return_both, return_residual)
 
     def _attention(self, L, h, fb: ForwardBatch, kv, li: int, attn: torch.Tensor) -> torch.Tensor:
@@ -625,10 +627,23 @@ class DecoderLM:
         qkv[:, H * D:(H + KVH) * D] = k
         return qkv
 
-    def _norm(self, x, delta, w, b=None):
+    def _post_norm(self, delta, post):
+        """The block's output norm by itself (models without one: delta as it is)."""
+        cfg = self.cfg
+        return delta if post is None else ops.rmsnorm(delta, post, cfg.rms_norm_eps, cfg.norm_offset_one)
+
+    def _norm(self, x, delta, w, b=None, post=None):
         """x <- x + delta; the block's input norm (RMSNorm, or LayerNorm with bias).
+        `post`: the previous block's output norm, which delta passes first; both
+        norms and the add are one launch, rounded where separate ones round.
         Blocks without input norms (OLMo 2/3, EXAONE 4) get the residual stream itself."""
         cfg = self.cfg
+        if post is not None and delta is not None:
+            if cfg.norm_kind != "layernorm" and delta.dtype == post.dtype == x.dtype and (w is None or w.dtype == x.dtype):
+                h = ops.block_norms(x, delta, post, w, cfg.rms_norm_eps, offset_one=cfg.norm_offset_one,
+                                    round_branch=True, inplace=True)[1]
+                return x if h is None else h
+            delta = self._post_norm(delta, post)
         if w is None and not cfg.pre_norms:
             if delta is not None:
                 x.add_(delta)
@@ -768,9 +783,10 @@ class DecoderLM:
         p0 = cache.offset
         positions = torch.arange(p0, p0 + Lq, dtype=torch.int32, device=tokens.device)
         x = ops.embedding(tokens.to(torch.int32), self.embed, cfg.embed_scale)
-        delta = None
+        delta = post = None
         for li, L in enumerate(self.layers):
-            h = self._norm(x, delta, L.ln1, L.ln1_b)
+            h = self._norm(x, delta, L.ln1, L.ln1_b, post)
+            post = None
             if L.block == "ffn":
                 delta = self._mlp(L, h)
                 continue
@@ -814,16 +830,14 @@ class DecoderLM:
             if cfg.parallel_block:
                 delta = (delta.float() + self._mlp(L, h).float()).to(x.dtype)
                 continue
-            if L.post_attn_norm is not None:
-                delta = ops.rmsnorm(delta, L.post_attn_norm, cfg.rms_norm_eps, cfg.norm_offset_one)
+            post = L.post_attn_norm
             if L.block == "mixer":
                 continue
-            h = self._norm(x, delta, L.ln2, L.ln2_b)
+            h = self._norm(x, delta, L.ln2, L.ln2_b, post)
             delta = self._mlp(L, h)
-            if L.post_ffn_norm is not None:
-                delta = ops.rmsnorm(delta, L.post_ffn_norm, cfg.rms_norm_eps, cfg.norm_offset_one)
+            post = L.post_ffn_norm
         cache.offset += Lq
-        h = self._norm(x, delta, self.norm, self.norm_b)
+        h = self._norm(x, delta, self.norm, self.norm_b, post)
         if return_hidden:
             return h
         return self._final_logits(h)

@@ -244,11 +244,12 @@ class Gemma4LM(DecoderLM):
         w = w.float() * L.g4_expert_scale.float()[idx.long()]
         return w, idx
 
-    def _ffn(self, L, x):
-        """The layer's feed-forward delta (before post_ffn_norm) for residual x."""
+    def _ffn(self, L, x, h=None):
+        """The layer's feed-forward delta (before post_ffn_norm) for residual x; h: ln2(x) where the caller has it."""
         cfg = self.cfg
         eps = cfg.rms_norm_eps
-        h = ops.rmsnorm(x, L.ln2, eps)
+        if h is None:
+            h = ops.rmsnorm(x, L.ln2, eps)
         m = ops.gemm(ops.gemm(h, L.wgu, epi=cfg.glu_epi), L.wd)
         if L.router is None:
             return m
@@ -264,12 +265,12 @@ class Gemma4LM(DecoderLM):
     def _block_tail(self, L, li, x, attn_out, ple):
         """Everything after attention: residual adds, FFN, per-layer input, scalar."""
         eps = self.cfg.rms_norm_eps
-        x = (x.float() + ops.rmsnorm(attn_out, L.post_attn_norm, eps).float()).to(x.dtype)
-        x = (x.float() + ops.rmsnorm(self._ffn(L, x), L.post_ffn_norm, eps).float()).to(x.dtype)
+        x, h = ops.block_norms(x, attn_out, L.post_attn_norm, L.ln2, eps, round_branch=True)
+        x, _ = ops.block_norms(x, self._ffn(L, x, h), L.post_ffn_norm, None, eps, round_branch=True)
         if ple is not None:
             gt = ops.gemm(x, L.ple_gate, epi="gelu_tanh")
             gt = (gt.float() * ple[:, li].float()).to(x.dtype)
-            x = (x.float() + ops.rmsnorm(ops.gemm(gt, L.ple_proj), L.ple_norm, eps).float()).to(x.dtype)
+            x, _ = ops.block_norms(x, ops.gemm(gt, L.ple_proj), L.ple_norm, None, eps, round_branch=True)
         return (x.float() * L.layer_scalar.float()).to(x.dtype)
 
     def _qkv_parts(self, L, li, h):

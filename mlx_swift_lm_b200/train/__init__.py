@@ -1,4 +1,5 @@
-"""Adapter training (plain-PyTorch autograd forward over the frozen model)."""
-from .forward import TrainableLoRA, train_forward  # noqa: F401
+"""Adapter training: an autograd forward over the frozen model, in plain PyTorch or
+(``TrainParameters.fused``) on the training operators."""
+from .forward import MaskStream, TrainableLoRA, train_forward, train_hidden  # noqa: F401
 from .lora_train import (Progress, TrainParameters, evaluate, iterate_batches, load_lora_data,  # noqa: F401
                          load_lora_file, loss_fn, train)

@@ -10,12 +10,17 @@ Parity: LoRALinear.callAsFunction (LoRA+Layers.swift:109: y + s * (dropout(x) A)
 and DoRA's forward (DoRA+Layers.swift:13, norm of the adapted weight held
 constant for the gradient).
 Dense decoders with tensor-parallel world 1 only.
+
+:func:`train_hidden` is the same forward up to the final norm on the training
+operators (``ops.block_norms``, ``ops.dropout``), for a loss that takes the hidden
+rows and the head (``ops.linear_cross_entropy``): no logits, no stored dropout masks.
 """
 from __future__ import annotations
 
 import torch
 import torch.nn.functional as Fn
 
+from .. import ops
 from ..adapters.lora import LoRAContainer
 from ..ops.reference import apply_rope_ref, attention_rows_ref
 
@@ -33,6 +38,19 @@ def _rms(x, w, eps, offset_one=False):
     return xf * inv * ww
 
 
+class MaskStream:
+    """Dropout masks of one training step: call i draws the mask of (seed, step, i),
+    so a step's masks are the same whenever it is run or resumed."""
+
+    def __init__(self, seed: int, step: int):
+        self.seed, self.step, self.calls = int(seed), int(step), 0
+
+    def dropout(self, x, p: float):
+        offset = (self.step << 24) + self.calls
+        self.calls += 1
+        return ops.dropout(x, p, self.seed, offset)
+
+
 class TrainableLoRA:
     """Adapter matrices of a :class:`LoRAContainer` as trainable leaves."""
 
@@ -41,6 +59,7 @@ class TrainableLoRA:
         self.scale = adapter.configuration.lora_parameters.scale
         self.dropout = adapter.configuration.lora_parameters.dropout
         self.dora = adapter.configuration.fine_tune_type == "dora"
+        self.masks: MaskStream | None = None  # counter-based dropout masks; None: torch's generator
         self.params: dict = {}
         for key, ent in adapter.tensors.items():
             a = ent["a"].to(device).float().requires_grad_(True)
@@ -69,7 +88,12 @@ class TrainableLoRA:
     def delta(self, x, key, w_rows, training: bool):
         """(s * dropout(x) A^T B^T, DoRA column scale or None) for one projection."""
         ent = self.params[key]
-        xd = Fn.dropout(x, self.dropout, training) if self.dropout > 0 else x
+        xd = x
+        if self.dropout > 0:
+            if self.masks is None:
+                xd = Fn.dropout(x, self.dropout, training)
+            elif training:
+                xd = self.masks.dropout(x, self.dropout)
         z = (xd @ ent["a"].t()) @ ent["b"].t() * self.scale
         if not self.dora:
             return z, None
@@ -140,14 +164,35 @@ def _mlp(model, L, li, x, lora, training):
     return _proj_plain(L.wd, L.bd, a, lora, (li, "mlp.down_proj"), training)
 
 
-def train_forward(model, tokens: torch.Tensor, lora: TrainableLoRA | None = None, training: bool = True):
-    """tokens [B, S] int64 -> logits [B, S, V] fp32, differentiable in the
-    LoRA parameters."""
-    cfg = model.cfg
+def _check_trainable(model):
     if model.tp.world != 1:
         raise ValueError("adapter training runs with tensor-parallel world 1")
     if any(L.moe for L in model.layers):
         raise ValueError("adapter training supports dense decoders")
+
+
+def _attention(model, L, li, h, pos, cs, lora, training):
+    """The attention block's output for the normed rows h [S, H] of one sequence."""
+    cfg, S = model.cfg, h.shape[0]
+    qkv = _proj_qkv(model, L, li, h, lora, training)
+    qn, kn = model.H * model.D, model.KVH * model.D
+    q = qkv[:, :qn].reshape(S, model.H, model.D)
+    k = qkv[:, qn:qn + kn].reshape(S, model.KVH, model.D)
+    v = qkv[:, qn + kn:].reshape(S, model.KVH, model.D)
+    if L.q_norm is not None:
+        q = _rms(q, L.q_norm, cfg.rms_norm_eps, cfg.norm_offset_one)
+        k = _rms(k, L.k_norm, cfg.rms_norm_eps, cfg.norm_offset_one)
+    q = apply_rope_ref(q, pos, cs, model.rot_dim, cfg.rope_interleaved)
+    k = apply_rope_ref(k, pos, cs, model.rot_dim, cfg.rope_interleaved)
+    a = attention_rows_ref(q, k, v, pos, S, cfg.scale, cfg.window(li), L.sinks, cfg.attn_logit_softcap)
+    return _proj_plain(L.wo, L.bo, a.reshape(S, -1), lora, (li, "self_attn.o_proj"), training)
+
+
+def train_forward(model, tokens: torch.Tensor, lora: TrainableLoRA | None = None, training: bool = True):
+    """tokens [B, S] int64 -> logits [B, S, V] fp32, differentiable in the
+    LoRA parameters."""
+    cfg = model.cfg
+    _check_trainable(model)
     B, S = tokens.shape
     dev = model.embed.device
     tokens = tokens.to(dev)
@@ -158,18 +203,7 @@ def train_forward(model, tokens: torch.Tensor, lora: TrainableLoRA | None = None
         x = model.embed[tokens[bi]].float() * cfg.embed_scale
         for li, L in enumerate(model.layers):
             h = _rms(x, L.ln1, cfg.rms_norm_eps, cfg.norm_offset_one)
-            qkv = _proj_qkv(model, L, li, h, lora, training)
-            qn, kn = model.H * model.D, model.KVH * model.D
-            q = qkv[:, :qn].reshape(S, model.H, model.D)
-            k = qkv[:, qn:qn + kn].reshape(S, model.KVH, model.D)
-            v = qkv[:, qn + kn:].reshape(S, model.KVH, model.D)
-            if L.q_norm is not None:
-                q = _rms(q, L.q_norm, cfg.rms_norm_eps, cfg.norm_offset_one)
-                k = _rms(k, L.k_norm, cfg.rms_norm_eps, cfg.norm_offset_one)
-            q = apply_rope_ref(q, pos, cs, model.rot_dim, cfg.rope_interleaved)
-            k = apply_rope_ref(k, pos, cs, model.rot_dim, cfg.rope_interleaved)
-            a = attention_rows_ref(q, k, v, pos, S, cfg.scale, cfg.window(li), L.sinks, cfg.attn_logit_softcap)
-            d = _proj_plain(L.wo, L.bo, a.reshape(S, -1), lora, (li, "self_attn.o_proj"), training)
+            d = _attention(model, L, li, h, pos, cs, lora, training)
             if L.post_attn_norm is not None:
                 d = _rms(d, L.post_attn_norm, cfg.rms_norm_eps, cfg.norm_offset_one)
             x = x + d
@@ -185,3 +219,26 @@ def train_forward(model, tokens: torch.Tensor, lora: TrainableLoRA | None = None
             lg = torch.tanh(lg / c) * c
         outs.append(lg)
     return torch.stack(outs)
+
+
+def train_hidden(model, tokens: torch.Tensor, lora: TrainableLoRA | None = None, training: bool = True):
+    """tokens [B, S] int64 -> final-normed rows [B, S, H] fp32, differentiable in
+    the LoRA parameters: :func:`train_forward` up to the head, with the norms
+    around each block, their residual add and the norm before the next one as one
+    operator over the whole batch."""
+    cfg = model.cfg
+    _check_trainable(model)
+    B, S = tokens.shape
+    dev = model.embed.device
+    pos = torch.arange(S, device=dev)
+    cs = model.cos_sin.to(dev)
+    f32 = lambda w: None if w is None else w.float()  # noqa: E731
+    x = model.embed[tokens.to(dev).reshape(-1)].float() * cfg.embed_scale
+    h = _rms(x, model.layers[0].ln1, cfg.rms_norm_eps, cfg.norm_offset_one)
+    for li, L in enumerate(model.layers):
+        d = torch.cat([_attention(model, L, li, h[b * S:(b + 1) * S], pos, cs, lora, training) for b in range(B)])
+        x, h = ops.block_norms(x, d, f32(L.post_attn_norm), f32(L.ln2), cfg.rms_norm_eps, offset_one=cfg.norm_offset_one)
+        d = _mlp(model, L, li, h, lora, training)
+        after = model.layers[li + 1].ln1 if li + 1 < len(model.layers) else model.norm
+        x, h = ops.block_norms(x, d, f32(L.post_ffn_norm), f32(after), cfg.rms_norm_eps, offset_one=cfg.norm_offset_one)
+    return h.reshape(B, S, -1)

@@ -9,6 +9,11 @@ adapter weights the container already holds.
 
 Loss: cross entropy of position j's logits against token j+1, counted only
 where token j+1 is a real token of the sample (padding never scores).
+
+With ``TrainParameters.fused`` the step runs on the training operators: the norms
+around the blocks, counter-based dropout (a step's masks follow from the seed and the
+step's number, resumed runs included) and the loss from the hidden rows without logits.
+On CUDA the head's product takes its rows in bf16 there.
 """
 from __future__ import annotations
 
@@ -22,8 +27,9 @@ from typing import Callable, Iterator
 import torch
 import torch.nn.functional as Fn
 
+from .. import ops
 from ..adapters.lora import LoRAContainer
-from .forward import TrainableLoRA, train_forward
+from .forward import MaskStream, TrainableLoRA, train_forward, train_hidden
 
 
 @dataclass
@@ -38,6 +44,7 @@ class TrainParameters:
     completed_iterations: int = 0
     learning_rate: float = 1e-5
     seed: int = 0
+    fused: bool = False  # run on ops.block_norms, ops.dropout and ops.linear_cross_entropy
 
     def __post_init__(self):
         if self.completed_iterations < 0:
@@ -106,11 +113,20 @@ def iterate_batches(dataset: list[str], tokenizer, batch_size: int, train: bool,
         yield arr[:, :-1], arr[:, 1:], torch.tensor(lengths)
 
 
-def loss_fn(model, lora: TrainableLoRA | None, inputs, targets, lengths, training=True):
-    """(mean loss over scored tokens, number of scored tokens)."""
-    logits = train_forward(model, inputs, lora, training)
+def loss_fn(model, lora: TrainableLoRA | None, inputs, targets, lengths, training=True, fused=False):
+    """(mean loss over scored tokens, number of scored tokens). `fused`: from the
+    hidden rows and the head, without logits."""
     S = inputs.shape[1]
     mask = torch.arange(S)[None, :] < (lengths[:, None] - 1)
+    if fused:
+        h = train_hidden(model, inputs, lora, training)
+        if not isinstance(model.lm_head, torch.Tensor):
+            raise ValueError("the fused loss needs a dense head")
+        scored = torch.where(mask, targets, -100).to(h.device)
+        loss = ops.linear_cross_entropy(h.to(model.lm_head.dtype), model.lm_head, scored,
+                                        softcap=model.cfg.final_logit_softcap, reduction="mean")
+        return loss, int(mask.sum())
+    logits = train_forward(model, inputs, lora, training)
     mask = mask.to(logits.device)
     ce = Fn.cross_entropy(logits.reshape(-1, logits.shape[-1]), targets.to(logits.device).reshape(-1),
                           reduction="none").reshape(mask.shape)
@@ -119,12 +135,12 @@ def loss_fn(model, lora: TrainableLoRA | None, inputs, targets, lengths, trainin
 
 
 @torch.no_grad()
-def evaluate(model, lora, dataset, tokenizer, batch_size, batches=0):
+def evaluate(model, lora, dataset, tokenizer, batch_size, batches=0, fused=False):
     tot, ntok = 0.0, 0
     for k, (x, y, ln) in enumerate(iterate_batches(dataset, tokenizer, batch_size, train=False)):
         if batches and k >= batches:
             break
-        l, n = loss_fn(model, lora, x, y, ln, training=False)
+        l, n = loss_fn(model, lora, x, y, ln, training=False, fused=fused)
         tot += float(l) * n
         ntok += n
     return tot / max(ntok, 1)
@@ -143,7 +159,9 @@ def train(model, adapter: LoRAContainer, tokenizer, train_set: list[str], valid_
     start = params.completed_iterations
     for step in range(start, params.iterations):
         x, y, ln = next(it)
-        loss, n = loss_fn(model, lora, x, y, ln, training=True)
+        if params.fused:
+            lora.masks = MaskStream(params.seed, step)
+        loss, n = loss_fn(model, lora, x, y, ln, training=True, fused=params.fused)
         opt.zero_grad(set_to_none=True)
         loss.backward()
         opt.step()
@@ -158,7 +176,7 @@ def train(model, adapter: LoRAContainer, tokenizer, train_set: list[str], valid_
             if progress and progress(ev) is False:
                 break
         if valid_set and (i == 1 or i % params.steps_per_eval == 0):
-            vl = evaluate(model, lora, valid_set, tokenizer, params.batch_size, params.validation_batches)
+            vl = evaluate(model, lora, valid_set, tokenizer, params.batch_size, params.validation_batches, params.fused)
             if progress and progress(Progress("validation", i, vl)) is False:
                 break
         if params.adapter_path and i % params.save_every == 0:
