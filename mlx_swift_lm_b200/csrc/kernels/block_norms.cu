@@ -89,8 +89,10 @@ __device__ __forceinline__ void factors(float* w, const void* p, float one, floa
     Group<W, E> q;
     load_group<W, VEC, E>(q, reinterpret_cast<const W*>(p), v, threads, H);
     q.unpack(w);
+    if (one != 0.f) {
 #pragma unroll
-    for (int j = 0; j < E; ++j) w[j] += one;
+      for (int j = 0; j < E; ++j) w[j] += one;
+    }
   } else {
 #pragma unroll
     for (int j = 0; j < E; ++j) w[j] = none;
@@ -266,39 +268,37 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) block_norms_bwd_kernel(cons
     const void* gate = nullptr;  // a gate along the columns
     if (GATED && a.gate_kind == kGateChannel) gate = a.gate;
     if (GATED && a.gate_kind == kGateElement) gate = reinterpret_cast<const T*>(a.gate) + row * a.ldg;
-    float s[4] = {};
+    // r1 and r2 are factored out of the sums and of what the second loop repeats:
+    //   q = r2 dh pre, b = dy + q, c = delta post (gate);  dt = b - y r2^2 (sum q y) / H
+    float s[4] = {}, b[NV][E];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      float c[E], b[E], w[E], f[E];
+      float c[E], w[E], f[E], t[E];
       d[v].unpack(c);
       factors<W, VEC, E>(w, a.post, one, 1.f, v, n, H);
 #pragma unroll
-      for (int j = 0; j < E; ++j) c[j] *= r1 * w[j];
+      for (int j = 0; j < E; ++j) c[j] *= w[j];
       if (GATED) {
         factors<T, VEC, E>(w, gate, 0.f, 1.f, v, n, H);
 #pragma unroll
         for (int j = 0; j < E; ++j) c[j] *= w[j];
       }
-      ty[v].unpack(b);
+      ty[v].unpack(b[v]);
+      y[v].unpack(f);
+      th[v].unpack(t);
       factors<W, VEC, E>(w, pre, one, 0.f, v, n, H);
-      float yh[E];
-      y[v].unpack(yh);
-      th[v].unpack(f);
 #pragma unroll
       for (int j = 0; j < E; ++j) {
-        const float t = yh[j] * r2, g = f[j] * w[j];
-        cpre[v][j] += f[j] * t;
-        s[0] += g * t;
-        s[1] += c[j] * (b[j] + r2 * g);
-        s[2] += c[j] * t;
+        t[j] *= r2;
+        cpre[v][j] += t[j] * f[j];
+        const float q = t[j] * w[j];
+        b[v][j] += q;
+        s[0] += q * f[j];
+        s[1] += c[j] * b[v][j];
+        s[2] += c[j] * f[j];
       }
-    }
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
       y[v].hold();
       d[v].hold();
-      ty[v].hold();
-      th[v].hold();
     }
     const float t = warp_sum4(s);
     if ((lane & 7) == 0) red[flip][lane >> 3][wid] = t;
@@ -310,58 +310,49 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) block_norms_bwd_kernel(cons
     const float total = warp_sum4(q);
     const float s1 = __shfl_sync(0xffffffffu, total, 0), s2 = __shfl_sync(0xffffffffu, total, 8),
                 s3 = __shfl_sync(0xffffffffu, total, 16);
-    const float m = r2 * s1 * inv_h;              // dt = b - m yhat
-    const float along = a.scale * (s2 - m * s3);  // sum of scale * dt * c, without a row gate
-    const float m1 = a.post ? along * grow * inv_h : 0.f;
+    const float mr2 = s1 * inv_h * r2 * r2;
+    const float k1 = r1 * a.scale;
+    const float along = k1 * (s2 - mr2 * s3);  // sum of scale * dt * dhat * post, without a row gate
+    const float k2 = a.post ? r1 * r1 * (along * grow * inv_h) : 0.f;
     if (GATED && a.gate_kind == kGateRow && a.dgate && threadIdx.x == 0)
       reinterpret_cast<T*>(a.dgate)[row] = from_f32<T>(along);
-    const float mr2 = m * r2;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      float dt[E], w[E], f[E];
-      ty[v].unpack(dt);
-      factors<W, VEC, E>(w, pre, one, 0.f, v, n, H);
-      th[v].unpack(f);
-#pragma unroll
-      for (int j = 0; j < E; ++j) dt[j] += r2 * (f[j] * w[j]);
+      float w[E], f[E];
+      Group<T, E> o;
       y[v].unpack(f);
 #pragma unroll
-      for (int j = 0; j < E; ++j) dt[j] -= f[j] * mr2;
+      for (int j = 0; j < E; ++j) b[v][j] -= f[j] * mr2;  // dt
       if (a.dx) {
-        ty[v].pack(dt);
-        store_group<T, VEC, E>(reinterpret_cast<T*>(a.dx) + row * a.ldo, ty[v], v, n, H);
+        o.pack(b[v]);
+        store_group<T, VEC, E>(reinterpret_cast<T*>(a.dx) + row * a.ldo, o, v, n, H);
       }
       factors<W, VEC, E>(w, a.post, one, 1.f, v, n, H);
       d[v].unpack(f);
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        f[j] *= r1;  // dhat
-        dt[j] *= a.scale;
-      }
+      for (int j = 0; j < E; ++j) b[v][j] *= k1;
       if (GATED) {
-        float g[E];
+        float g[E], dg[E];
         factors<T, VEC, E>(g, gate, 0.f, grow, v, n, H);
-        float dg[E];
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-          dg[j] = dt[j] * f[j] * w[j];
+          dg[j] = b[v][j] * f[j] * w[j];
           cgate[v][j] += dg[j];
-          dt[j] *= g[j];
+          b[v][j] *= g[j];
         }
         if (a.gate_kind == kGateElement && a.dgate) {
-          Group<T, E> o;
           o.pack(dg);
           store_group<T, VEC, E>(reinterpret_cast<T*>(a.dgate) + row * a.ldo, o, v, n, H);
         }
       }
 #pragma unroll
       for (int j = 0; j < E; ++j) {
-        cpost[v][j] += dt[j] * f[j];
-        dt[j] = r1 * (dt[j] * w[j] - f[j] * m1);
+        cpost[v][j] += b[v][j] * f[j];
+        b[v][j] = b[v][j] * w[j] - k2 * f[j];
       }
       if (a.ddelta) {
-        d[v].pack(dt);
-        store_group<T, VEC, E>(reinterpret_cast<T*>(a.ddelta) + row * a.ldo, d[v], v, n, H);
+        o.pack(b[v]);
+        store_group<T, VEC, E>(reinterpret_cast<T*>(a.ddelta) + row * a.ldo, o, v, n, H);
       }
     }
   }
