@@ -25,7 +25,7 @@
 // either operand's rows and half of the accumulator's). Per CTA, warp 0 fetches its
 // operand halves by TMA into a ring of 64-deep stages, one thread of the pair issues
 // the MMAs into one of two accumulators in tensor memory (2 x 256 columns), and warps
-// 4 - 7 work on the other one's finished tile, a row of it per thread: the softmax
+// 4 - 11 work on the other one's finished tile, half a row of it per thread: the softmax
 // arithmetic and the stores run under the next tile's product. Tiles leave through
 // shared memory by TMA; the fp32 sums of dh are added up in L2 by its reduction.
 #include "b200_common.cuh"
@@ -68,12 +68,13 @@ struct Args {
 constexpr int kTileM = 256, kTileN = 256, kStages = 6;  // of a pair of CTAs
 constexpr int kRowsM = kTileM / 2, kRowsN = kTileN / 2;   // a CTA's share of either operand
 constexpr int kABytes = kRowsM * 128, kBBytes = kRowsN * 128, kStageBytes = kABytes + kBBytes;
-constexpr int kOutBytes = kRowsM * 128;  // one of two staging buffers: 128 rows of 128 bytes
+constexpr int kOutBytes = kRowsM * 128;  // a staging buffer for each half of the columns: 128 rows of 128 bytes
 constexpr int kBars = 2 * kStages + 4;
 constexpr int kBarOffset = kStages * kStageBytes + 2 * kOutBytes;
-constexpr int kSmem = kBarOffset + kBars * 8 + 16 + 1024;
-constexpr int kThreads = 256;
-constexpr int kEpiWarps = 4;
+constexpr int kSmem = kBarOffset + kBars * 8 + 16 + 1024;  // kStats keeps its pairs in the staging buffers
+constexpr int kThreads = 384;
+constexpr int kEpiWarps = 8;  // two for each quarter of the lanes: one takes the left half of the columns, one the right
+constexpr int kHalfN = kTileN / 2;
 constexpr int kGroupM = 16;  // row tiles walked per column tile before the next: W is read once per 16 x 256 rows, h stays in L2
 static_assert(kSmem <= 227 * 1024, "shared memory plan exceeds the per-CTA limit");
 
@@ -143,7 +144,9 @@ __device__ __forceinline__ void bulk_wait_read() {
   asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-__device__ __forceinline__ void epi_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory"); }
+// Barrier of the four warps of one half of the columns (ids 1 and 2), and of all eight (3).
+__device__ __forceinline__ void half_barrier(int half) { asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory"); }
+__device__ __forceinline__ void epi_barrier() { asm volatile("bar.sync 3, %0;" ::"n"(32 * kEpiWarps) : "memory"); }
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -176,6 +179,17 @@ __device__ __forceinline__ int choose_parts(int tiles, int kb, int pairs, int mo
 // rounded to bf16 (the losses take tanhf); 5 instructions for about 20.
 __device__ __forceinline__ float tanh_fast(float x) {
   return 1.f - __fdividef(2.f, 1.f + ex2(2.f * kLog2e * x));
+}
+
+// (max, sum of exp) of two sets of logits as one.
+__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
+  const float top = fmaxf(m, m2);
+  if (top > -INFINITY) {
+    s = s * (m > -INFINITY ? ex2((m - top) * kLog2e) : 1.f) + s2 * (m2 > -INFINITY ? ex2((m2 - top) * kLog2e) : 1.f);
+    m = top;
+  } else {
+    s += s2;
+  }
 }
 
 // The tile walk of one launch: `mt` x `nt` tiles (times `splits` of the
@@ -342,10 +356,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
   } else if (warp >= 4) {
     const int r = (warp & 3) * 32 + lane;  // row of the CTA's half tile = tensor-memory lane
+    const int half = (warp - 4) >> 2, left = half * kHalfN;
+    const bool first_thread = (threadIdx.x & 127) == 0;  // of the half
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const float inv_n = 1.f / (float)max(n, 1);
     const uint32_t release = in_leader(bar_tempty);
-    int tile = 0, out = 0;
+    int tile = 0;
+    bool dead = false;
     for (int t = pair; t < w.total; t += pairs, ++tile) {
       int m, nn, s;
       w.at(t, m, nn, s);
@@ -354,6 +371,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const uint32_t acc = tmem + lanes + buf * kTileN;
       const bool empty = s * kb_per >= kb_total;  // nothing contracted: the product is zero
       const int cols = min(kTileN, (OP == kStats || OP == kGrad ? a.nv : a.K) - n0);
+      const int end = min(left + kHalfN, cols);  // this half: columns left .. end - 1 of the tile, or none
       int target = -1;
       float shift = 0.f, dl = 0.f, at_target = 0.f;
       if constexpr (OP == kStats || OP == kGrad) {
@@ -366,13 +384,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
         }
       }
-      const bool ok = mbar_wait(bar_tfull + 8 * buf, (tile >> 1) & 1, kErrTmemWait);
-      if (!__all_sync(0xffffffffu, ok)) break;
+      // after a wait that ran out (the status word says so) the warp goes on without waiting, so
+      // that the barriers among the warps are all met and the kernel ends
+      if (!dead) dead = __any_sync(0xffffffffu, !mbar_wait(bar_tfull + 8 * buf, (tile >> 1) & 1, kErrTmemWait));
       tc_fence_after();
       if constexpr (OP == kStats) {
         float mx = -INFINITY, sum = 0.f;
 #pragma unroll 1
-        for (int c = 0; c < cols; c += 32) {
+        for (int c = left; c < end; c += 32) {
           uint32_t v[32];
           tmem_ld32(acc + c, v);
           tc_wait_ld();
@@ -410,14 +429,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) arrive_cluster(release + 8 * buf);
-        if (row < n) a.part[(int64_t)nn * a.T + row] = make_float2(mx, sum);
+        // the right half's pair joins the left's; the buffers alternate between tiles, and the barrier
+        // of the next tile is passed before one is written again
+        float2* pairs_smem = reinterpret_cast<float2*>(smem + kStages * kStageBytes) + (tile & 1) * kRowsM;
+        if (half) pairs_smem[r] = make_float2(mx, sum);
+        epi_barrier();
+        if (!half && row < n) {
+          const float2 p = pairs_smem[r];
+          join(mx, sum, p.x, p.y);
+          a.part[(int64_t)nn * a.T + row] = make_float2(mx, sum);
+        }
       } else {
-        // 128 bytes of a row at a time (64 bf16 or 32 fp32) through one of two staging buffers
-        // in the 128-byte swizzle, stored by one thread while the next ones are filled
+        // 128 bytes of a row at a time (64 bf16 or 32 fp32) through the half's staging buffer in the
+        // 128-byte swizzle, stored by one thread while the next ones are formed
         constexpr int kStep = OP == kDh ? 32 : 64;
         const bool any_row = OP == kDw ? m0 < a.nv : m0 < n;
 #pragma unroll 1
-        for (int c = 0; c < cols; c += kStep, ++out) {
+        for (int c = left; c < end; c += kStep) {
           uint32_t o[32];
           if constexpr (OP == kGrad) {
 #pragma unroll
@@ -462,17 +490,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int j = 0; j < 32; ++j) o[j] = 0u;
           }
-          const uint32_t stage = out_smem + (out & 1) * kOutBytes;
-          if (threadIdx.x == 128) bulk_wait_read<1>();  // the store before last has left this buffer
-          epi_barrier();
+          const uint32_t stage = out_smem + half * kOutBytes;
+          if (first_thread) bulk_wait_read<0>();  // the last store has left the buffer
+          half_barrier(half);
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + sw128_offset(r, 16 * j)), "r"(o[4 * j]),
                          "r"(o[4 * j + 1]), "r"(o[4 * j + 2]), "r"(o[4 * j + 3])
                          : "memory");
           fence_proxy_async_smem();
-          epi_barrier();
-          if (threadIdx.x == 128) {
+          half_barrier(half);
+          if (first_thread) {
             if (any_row) {  // a box that starts inside; what reaches past the end is not written
               if constexpr (OP == kGrad) tma_store(&tmO, stage, n0 + c, m0);
               else if constexpr (OP == kDw) tma_store(&tmO, stage, n0 + c, a.v0 + m0);
@@ -487,7 +515,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (lane == 0) arrive_cluster(release + 8 * buf);
       }
     }
-    if (OP != kStats && threadIdx.x == 128) bulk_wait_all();
+    if (OP != kStats && first_thread) bulk_wait_all();
   }
   __syncwarp();
   tc_fence_before();
@@ -612,16 +640,6 @@ struct MergeArgs {
   int T, nt, mean;
 };
 constexpr int kMergeWarps = 32;
-
-__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
-  const float top = fmaxf(m, m2);
-  if (top > -INFINITY) {
-    s = s * (m > -INFINITY ? ex2((m - top) * kLog2e) : 1.f) + s2 * (m2 > -INFINITY ? ex2((m2 - top) * kLog2e) : 1.f);
-    m = top;
-  } else {
-    s += s2;
-  }
-}
 
 __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(MergeArgs a) {
   pdl_launch_dependents();
