@@ -156,11 +156,13 @@ __device__ __forceinline__ float ex2(float x) {
 
 // Parts of dh's contraction of `kb` blocks of 64 over `tiles` output tiles: the
 // fewest that minimise the rounds of the CTA pairs times their length, so that few
-// rows still fill the machine and the last round is not half empty. A part costs
-// about kPartBlocks blocks beyond its product (its tile's way out). Chosen on the
-// device, where the number of scored rows is known, by a whole warp: a lane weighs
-// two of the at most kMostParts choices.
+// rows still fill the machine and the last round is not half empty. A part's tile
+// costs about kPartBlocks blocks on its way out, and its fp32 sums are written and
+// read once (512 KB a tile at 5 TB/s are kPartTraffic of the 0.37 us of a block).
+// Chosen on the device, where the number of scored rows is known, by a whole warp: a
+// lane weighs two of the at most kMostParts choices.
 constexpr int kPartBlocks = 6, kMostParts = 64;
+constexpr float kPartTraffic = 0.28f;
 __device__ __forceinline__ int choose_parts(int tiles, int kb, int pairs, int most) {
   unsigned best = 0xFFFFFFFFu;
 #pragma unroll
@@ -168,7 +170,7 @@ __device__ __forceinline__ int choose_parts(int tiles, int kb, int pairs, int mo
     const int s = (threadIdx.x & 31) + 32 * i + 1;
     if (s <= most && (s == 1 || kb >= 16 * s)) {
       const float rounds = ceilf((float)tiles * (float)s / (float)pairs);
-      const float cost = rounds * (float)((kb + s - 1) / s + kPartBlocks);
+      const float cost = rounds * (float)((kb + s - 1) / s + kPartBlocks) + kPartTraffic * (float)tiles * (float)s;
       best = min(best, (unsigned)fminf(cost, 6e7f) * kMostParts + (unsigned)(s - 1));  // the fewer win a tie
     }
   }
@@ -690,7 +692,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(MergeArgs a) {
 // ignored rows. e is what the target's entry of G lost when it was rounded to bf16:
 // that entry alone is of the size of the whole row, the others are far below it, so
 // with it added back the rounding of G hardly shows in dh (measured against 64 bits:
-// 2.7e-3 -> 1.7e-3, the output's own rounding). A row a CTA.
+// 2.7e-3 -> 1.7e-3, the output's own rounding). A thread takes E columns of a row.
 struct FinishArgs {
   Args g;
   const float* acc;
@@ -698,51 +700,50 @@ struct FinishArgs {
   const __nv_bfloat16* w;
   __nv_bfloat16* dh;
   int64_t ldw;
-  int lda;  // row stride of acc
+  int lda;       // row stride of acc
+  int per_row;   // threads a row
 };
+template <int E>
 __global__ void __launch_bounds__(256) finish_dh_kernel(const FinishArgs a) {
   pdl_launch_dependents();
   pdl_wait();
-  const int t = blockIdx.x, K = a.g.K;
+  const int n = *a.g.count;
+  const int parts = dh_parts(a.g, n);
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int t = (int)(i / a.per_row);
+  if (t >= a.g.T) return;
+  const int c = (int)(i - (int64_t)t * a.per_row) * E;
   const int p = a.place[t];
-  __nv_bfloat16* o = a.dh + (int64_t)t * K;
-  float e = 0.f;
-  const __nv_bfloat16* wr = a.w;
+  __nv_bfloat16* o = a.dh + (int64_t)t * a.g.K + c;
+  float s[E] = {};
   if (p >= 0) {
-    const float g = target_grad(a.g, p, 1.f / (float)max(*a.g.count, 1));
-    e = g - bf2f(f2bf(g));
-    wr += (int64_t)max(a.g.target[p], 0) * a.ldw;
-  }
-  const float* row = a.acc + (int64_t)max(p, 0) * a.lda;
-  const int64_t part = (int64_t)a.g.acc_rows * a.lda;
-  const int parts = dh_parts(a.g, *a.g.count);
-  if (K % 8 == 0) {  // W's rows and acc's are 16-byte aligned whatever K is; dh's are if K is whole
-    for (int c = threadIdx.x * 8; c < K; c += 256 * 8) {
-      uint4 out = make_uint4(0, 0, 0, 0);
-      if (p >= 0) {
-        float s[8];
-        const uint4 wv = *reinterpret_cast<const uint4*>(wr + c);
-        const __nv_bfloat16* we = reinterpret_cast<const __nv_bfloat16*>(&wv);
+    const float g = target_grad(a.g, p, 1.f / (float)max(n, 1));
+    const float e = g - bf2f(f2bf(g));
+    const __nv_bfloat16* wr = a.w + (int64_t)max(a.g.target[p], 0) * a.ldw + c;
+    const float* row = a.acc + (int64_t)p * a.lda + c;
+    const int64_t part = (int64_t)a.g.acc_rows * a.lda;
+    if constexpr (E == 8) {
+      const uint4 wv = *reinterpret_cast<const uint4*>(wr);
+      const __nv_bfloat16* we = reinterpret_cast<const __nv_bfloat16*>(&wv);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[j] = e * bf2f(we[j]);
-        for (int k = 0; k < parts; ++k) {
-          const float4 x = *reinterpret_cast<const float4*>(row + k * part + c);
-          const float4 y = *reinterpret_cast<const float4*>(row + k * part + c + 4);
-          s[0] += x.x, s[1] += x.y, s[2] += x.z, s[3] += x.w;
-          s[4] += y.x, s[5] += y.y, s[6] += y.z, s[7] += y.w;
-        }
-        out = make_uint4(pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3]), pack_bf16x2(s[4], s[5]), pack_bf16x2(s[6], s[7]));
+      for (int j = 0; j < 8; ++j) s[j] = e * bf2f(we[j]);
+#pragma unroll 4
+      for (int k = 0; k < parts; ++k) {
+        const float4 x = *reinterpret_cast<const float4*>(row + k * part);
+        const float4 y = *reinterpret_cast<const float4*>(row + k * part + 4);
+        s[0] += x.x, s[1] += x.y, s[2] += x.z, s[3] += x.w;
+        s[4] += y.x, s[5] += y.y, s[6] += y.z, s[7] += y.w;
       }
-      *reinterpret_cast<uint4*>(o + c) = out;
-    }
-  } else {
-    for (int c = threadIdx.x; c < K; c += 256) {
-      float s = p >= 0 ? e * bf2f(wr[c]) : 0.f;
-      if (p >= 0)
-        for (int k = 0; k < parts; ++k) s += row[k * part + c];
-      o[c] = f2bf(s);
+    } else {
+      s[0] = e * bf2f(*wr);
+      for (int k = 0; k < parts; ++k) s[0] += row[k * part];
     }
   }
+  if constexpr (E == 8)
+    *reinterpret_cast<uint4*>(o) =
+        make_uint4(pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3]), pack_bf16x2(s[4], s[5]), pack_bf16x2(s[6], s[7]));
+  else
+    *o = f2bf(s[0]);
 }
 
 template <int OP>
@@ -935,7 +936,11 @@ int b200_lce_backward(void* saved, const void* W, int64_t ldw, const float* dlos
     q.ldw = ldw;
     q.dh = reinterpret_cast<__nv_bfloat16*>(dh);
     q.lda = lda;
-    cudaError_t e = launch_k(finish_dh_kernel, dim3((unsigned)T), dim3(256), 0, st, 1, q);
+    // vectors of eight where rows are whole ones (W's and the sums' rows are aligned whatever K is)
+    q.per_row = K % 8 == 0 ? K / 8 : K;
+    const int64_t blocks = tiles_of((int64_t)T * q.per_row, 256);
+    if (blocks > 0x7FFFFFFFll) return -1;
+    cudaError_t e = launch_k(K % 8 == 0 ? finish_dh_kernel<8> : finish_dh_kernel<1>, dim3((unsigned)blocks), dim3(256), 0, st, 1, q);
     if (e != cudaSuccess) return (int)e;
   }
   return (int)cudaGetLastError();
