@@ -45,6 +45,7 @@ struct BlockNormArgs {
   int gate_kind;
   int want_post, want_pre, want_gate;
   int offset_one, round_branch;
+  int slots;  // backward: rows that a stage holds (delta, and dy, y, dh, gate where given)
   float eps, scale;
 };
 
@@ -235,9 +236,105 @@ __global__ void __launch_bounds__(1024, 1) block_norms_kernel(const BlockNormArg
 // Both means come from one round of sums: with c = gate * post * dhat and
 // b = dy + r2 g, mean(w * dhat) = scale * (sum c b - r2 m sum c yhat) / H where
 // m = mean(g * yhat), so neither waits for the other.
-template <typename T, typename W, bool VEC, int NV, bool GATED, int MAXT>
-__global__ void __launch_bounds__(MAXT, 1024 / MAXT) block_norms_bwd_kernel(const BlockNormArgs a) {
+//
+// STAGES > 0: the rows arrive in shared memory by bulk copies, STAGES of them under
+// way at a time, so that a row's loads run under the sums of those before it and cost
+// no registers; those hold the weights instead. 0 (unaligned rows, and rows too wide
+// for two stages): straight from global memory. 8192 x 4096 bf16 (403 MB): 95 us from
+// global memory, 81 us (5.0 TB/s) staged, bound by the sums' round trips between rows.
+template <typename T, bool VEC, int E, int STAGES>
+struct BwdRows {
+  const BlockNormArgs& a;
+  int n, tid;
+  uint32_t ring, bars;  // shared memory: [STAGES][slots][row bytes], [STAGES] barriers
+  int slots, row_bytes;
+  bool dead = false;
+  uint32_t at = 0;      // the current row's stage
+  int64_t row = 0;
+
+  __device__ __forceinline__ BwdRows(const BlockNormArgs& args, uint8_t* smem)
+      : a(args), n(blockDim.x), tid(threadIdx.x), ring(smem_u32(smem)), bars(0), slots(args.slots),
+        row_bytes(args.H * (int)sizeof(T)) {
+    if constexpr (STAGES > 0) {
+      bars = ring + STAGES * slots * row_bytes;
+      if (tid == 0) {
+        for (int i = 0; i < STAGES; ++i) mbar_init(bars + 8 * i, 1);
+        fence_barrier_init();
+      }
+      __syncthreads();
+    }
+  }
+  // The k-th row of this CTA into its stage (one thread).
+  __device__ __forceinline__ void fetch(int k) {
+    const int64_t r = blockIdx.x + (int64_t)k * gridDim.x;
+    if (r >= a.T) return;
+    const uint32_t dst = ring + (k % (STAGES > 0 ? STAGES : 1)) * slots * row_bytes, bar = bars + 8 * (k % (STAGES > 0 ? STAGES : 1));
+    const uint64_t pol = l2_policy_evict_first();
+    mbar_arrive_expect_tx(bar, (uint32_t)(slots * row_bytes));
+    int s = 0;
+    auto get = [&](const void* p, int64_t ld) {
+      bulk_g2s(dst + row_bytes * s++, reinterpret_cast<const T*>(p) + r * ld, (uint32_t)row_bytes, bar, pol);
+    };
+    get(a.delta, a.ldd);
+    if (a.dy) get(a.dy, a.lddy);
+    if (a.dh) {
+      get(a.y, a.ldy);
+      get(a.dh, a.lddh);
+    }
+    if (a.gate_kind == kGateElement) get(a.gate, a.ldg);
+  }
+  __device__ __forceinline__ void begin(int k, int64_t r) {
+    row = r;
+    if constexpr (STAGES > 0) {
+      at = ring + (k % STAGES) * slots * row_bytes;
+      // after a wait that ran out (the status word says so) the rows go by unread waits, so that the kernel ends
+      if (!dead) dead = !mbar_wait(bars + 8 * (k % STAGES), (k / STAGES) & 1, kErrGemmWait);
+    }
+  }
+  __device__ __forceinline__ void load(Group<T, E>& g, int slot, const void* p, int64_t ld, int v) const {
+    if constexpr (STAGES > 0) {
+      const int c = column<true, E>(v, 0, n);
+      if (c < a.H) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(&g);
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                     : "r"(at + slot * row_bytes + c * (int)sizeof(T)));
+      } else {
+        g.zero();
+      }
+    } else {
+      load_group<T, VEC, E>(g, reinterpret_cast<const T*>(p) + row * ld, v, n, a.H);
+    }
+  }
+  __device__ __forceinline__ void delta(Group<T, E>& g, int v) const { load(g, 0, a.delta, a.ldd, v); }
+  __device__ __forceinline__ void dy(Group<T, E>& g, int v) const {
+    if (a.dy) load(g, 1, a.dy, a.lddy, v);
+    else g.zero();
+  }
+  __device__ __forceinline__ void y(Group<T, E>& g, int v) const {
+    if (a.dh) load(g, 1 + (a.dy != nullptr), a.y, a.ldy, v);
+    else g.zero();
+  }
+  __device__ __forceinline__ void dh(Group<T, E>& g, int v) const {
+    if (a.dh) load(g, 2 + (a.dy != nullptr), a.dh, a.lddh, v);
+    else g.zero();
+  }
+  // Gate along the columns (1 where there is none), times `by`.
+  __device__ __forceinline__ void gate(float* w, float by, int v) const {
+    if (a.gate_kind == kGateElement) {
+      Group<T, E> g;
+      load(g, slots - 1, a.gate, a.ldg, v);
+      g.unpack(w);
+    } else {
+      factors<T, VEC, E>(w, a.gate_kind == kGateChannel ? a.gate : nullptr, 0.f, by, v, n, a.H);
+    }
+  }
+};
+
+template <typename T, typename W, bool VEC, int NV, bool GATED, int MAXT, int STAGES>
+__global__ void __launch_bounds__(MAXT, STAGES > 0 ? 1 : 1024 / MAXT) block_norms_bwd_kernel(const BlockNormArgs a) {
   constexpr int E = 16 / sizeof(T);  // 16-byte groups
+  extern __shared__ __align__(128) uint8_t bwd_smem[];
   pdl_launch_dependents();
   pdl_wait();
   __shared__ float red[2][4][32];
@@ -245,48 +342,65 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) block_norms_bwd_kernel(cons
   const float one = a.offset_one ? 1.f : 0.f, inv_h = 1.f / (float)H;
   const void* pre = a.dh ? a.pre : nullptr;
   float cpost[NV][E] = {}, cpre[NV][E] = {}, cgate[GATED ? NV : 1][E] = {};
-  int flip = 0;
-  for (int64_t row = blockIdx.x; row < a.T; row += gridDim.x, flip ^= 1) {
+  int flip = 0, k = 0;
+  BwdRows<T, VEC, E, STAGES> rows(a, bwd_smem);
+  if (STAGES > 0 && threadIdx.x == 0)
+    for (int i = 0; i < STAGES; ++i) rows.fetch(i);
+  auto r1_of = [&](int64_t row) { return a.post && row < a.T ? a.r1[row] : 1.f; };
+  auto r2_of = [&](int64_t row) { return a.dh && row < a.T ? a.r2[row] : 0.f; };
+  float next_r1 = r1_of(blockIdx.x), next_r2 = r2_of(blockIdx.x);
+  // the weights stay in registers where the rows do not need them
+  float wpost[STAGES > 0 ? E : 1], wpre[STAGES > 0 ? E : 1];
+  if constexpr (STAGES > 0) {
+    factors<W, VEC, E>(wpost, a.post, one, 1.f, 0, n, H);
+    factors<W, VEC, E>(wpre, pre, one, 0.f, 0, n, H);
+  }
+  auto post_w = [&](float* w, int v) {
+    if constexpr (STAGES > 0) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) w[j] = wpost[j];
+    } else {
+      factors<W, VEC, E>(w, a.post, one, 1.f, v, n, H);
+    }
+  };
+  for (int64_t row = blockIdx.x; row < a.T; row += gridDim.x, flip ^= 1, ++k) {
     // the sums' buffers alternate between rows: a thread may be writing the next
     // row's while a slower one still reads this row's
-    Group<T, E> y[NV], d[NV], ty[NV], th[NV];
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      load_group<T, VEC, E>(d[v], reinterpret_cast<const T*>(a.delta) + row * a.ldd, v, n, H);
-      if (a.dh) {
-        load_group<T, VEC, E>(y[v], reinterpret_cast<const T*>(a.y) + row * a.ldy, v, n, H);
-        load_group<T, VEC, E>(th[v], reinterpret_cast<const T*>(a.dh) + row * a.lddh, v, n, H);
-      } else {
-        y[v].zero();
-        th[v].zero();
-      }
-      if (a.dy) load_group<T, VEC, E>(ty[v], reinterpret_cast<const T*>(a.dy) + row * a.lddy, v, n, H);
-      else ty[v].zero();
-    }
-    const float r1 = a.post ? a.r1[row] : 1.f, r2 = a.dh ? a.r2[row] : 0.f;
+    const float r1 = next_r1, r2 = next_r2;
+    next_r1 = r1_of(row + gridDim.x);
+    next_r2 = r2_of(row + gridDim.x);
     const float grow = GATED && a.gate_kind == kGateRow ? to_f32(reinterpret_cast<const T*>(a.gate)[row]) : 1.f;
-    const void* gate = nullptr;  // a gate along the columns
-    if (GATED && a.gate_kind == kGateChannel) gate = a.gate;
-    if (GATED && a.gate_kind == kGateElement) gate = reinterpret_cast<const T*>(a.gate) + row * a.ldg;
+    rows.begin(k, row);
+    Group<T, E> y[NV], d[NV];
     // r1 and r2 are factored out of the sums and of what the second loop repeats:
     //   q = r2 dh pre, b = dy + q, c = delta post (gate);  dt = b - y r2^2 (sum q y) / H
     float s[4] = {}, b[NV][E];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       float c[E], w[E], f[E], t[E];
+      Group<T, E> in;
+      rows.delta(d[v], v);
       d[v].unpack(c);
-      factors<W, VEC, E>(w, a.post, one, 1.f, v, n, H);
+      post_w(w, v);
 #pragma unroll
       for (int j = 0; j < E; ++j) c[j] *= w[j];
       if (GATED) {
-        factors<T, VEC, E>(w, gate, 0.f, 1.f, v, n, H);
+        rows.gate(w, 1.f, v);
 #pragma unroll
         for (int j = 0; j < E; ++j) c[j] *= w[j];
       }
-      ty[v].unpack(b[v]);
+      rows.dy(in, v);
+      in.unpack(b[v]);
+      rows.y(y[v], v);
       y[v].unpack(f);
-      th[v].unpack(t);
-      factors<W, VEC, E>(w, pre, one, 0.f, v, n, H);
+      rows.dh(in, v);
+      in.unpack(t);
+      if constexpr (STAGES > 0) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) w[j] = wpre[j];
+      } else {
+        factors<W, VEC, E>(w, pre, one, 0.f, v, n, H);
+      }
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         t[j] *= r2;
@@ -297,12 +411,16 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) block_norms_bwd_kernel(cons
         s[1] += c[j] * b[v][j];
         s[2] += c[j] * f[j];
       }
-      y[v].hold();
-      d[v].hold();
+      if (STAGES == 0) {
+        y[v].hold();
+        d[v].hold();
+      }
     }
     const float t = warp_sum4(s);
     if ((lane & 7) == 0) red[flip][lane >> 3][wid] = t;
     __syncthreads();
+    // every thread is done with the row before this one: its stage takes the row STAGES - 1 ahead
+    if (STAGES > 0 && threadIdx.x == 0 && k > 0) rows.fetch(k - 1 + STAGES);
     float q[4];
 #pragma unroll
     for (int k = 0; k < 3; ++k) q[k] = lane < nw ? red[flip][k][lane] : 0.f;
@@ -320,6 +438,10 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) block_norms_bwd_kernel(cons
     for (int v = 0; v < NV; ++v) {
       float w[E], f[E];
       Group<T, E> o;
+      if (STAGES > 0) {  // again from the stage rather than held over the sums
+        rows.y(y[v], v);
+        rows.delta(d[v], v);
+      }
       y[v].unpack(f);
 #pragma unroll
       for (int j = 0; j < E; ++j) b[v][j] -= f[j] * mr2;  // dt
@@ -327,13 +449,13 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) block_norms_bwd_kernel(cons
         o.pack(b[v]);
         store_group<T, VEC, E>(reinterpret_cast<T*>(a.dx) + row * a.ldo, o, v, n, H);
       }
-      factors<W, VEC, E>(w, a.post, one, 1.f, v, n, H);
+      post_w(w, v);
       d[v].unpack(f);
 #pragma unroll
       for (int j = 0; j < E; ++j) b[v][j] *= k1;
       if (GATED) {
         float g[E], dg[E];
-        factors<T, VEC, E>(g, gate, 0.f, grow, v, n, H);
+        rows.gate(g, grow, v);
 #pragma unroll
         for (int j = 0; j < E; ++j) {
           dg[j] = b[v][j] * f[j] * w[j];
@@ -438,30 +560,51 @@ static int launch_fwd(const BlockNormArgs& a, int num_sms, cudaStream_t st) {
 }
 
 // Backward: a 16-byte group a thread up to 1024 threads, more groups for wider rows.
-// Rows of at most 512 groups leave room for several CTAs on an SM, one's loads under
-// another's sums.
 static inline int bwd_threads(int H, int type) {
   const int g = type == kElemF32 ? (H + 3) / 4 : (H + 7) / 8;
   return round32(g < 1024 ? g : 1024);
 }
-template <typename T, typename W, bool VEC, bool GATED>
-static int launch_bwd_gate(const BlockNormArgs& a, int grid, cudaStream_t st) {
-  constexpr int E = 16 / sizeof(T), kWide = 32 / E;  // kWide x 1024 groups cover the widest row
-  const int groups = (a.H + E - 1) / E;
-  const dim3 threads(round32(groups < 1024 ? groups : 1024));
-  cudaError_t e;
-  if (groups > 1024)
-    e = launch_k(block_norms_bwd_kernel<T, W, VEC, kWide, GATED, 1024>, dim3(grid), threads, 0, st, 1, a);
-  else if (groups > 512)
-    e = launch_k(block_norms_bwd_kernel<T, W, VEC, 1, GATED, 1024>, dim3(grid), threads, 0, st, 1, a);
-  else
-    e = launch_k(block_norms_bwd_kernel<T, W, VEC, 1, GATED, 512>, dim3(grid), threads, 0, st, 1, a);
+// CTAs an SM by their registers a thread: 64, and at most 112 where the weights stay in
+// registers beside staged rows (512 threads or fewer).
+static inline int ctas_per_sm(int threads, int regs) {
+  const int c = 65536 / (regs * threads);
+  return c > 16 ? 16 : c < 1 ? 1 : c;
+}
+// Launches with at most `most` CTAs; returns their number in *grid.
+template <auto Kernel>
+static int launch_bwd_one(const BlockNormArgs& a, int64_t most, int threads, int smem, int* grid, cudaStream_t st) {
+  if (smem > 0)
+    if (int e = smem_attr_once<Kernel>(smem)) return e;
+  *grid = (int)(a.T < most ? a.T : most);
+  const cudaError_t e = launch_k(Kernel, dim3(*grid), dim3(threads), smem, st, 1, a);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
+template <typename T, typename W, bool VEC, bool GATED>
+static int launch_bwd_gate(const BlockNormArgs& a, int num_sms, int* grid, cudaStream_t st) {
+  constexpr int E = 16 / sizeof(T), kWide = 32 / E;  // kWide x 1024 groups cover the widest row
+  const int groups = (a.H + E - 1) / E;
+  const int threads = round32(groups < 1024 ? groups : 1024);
+  const int64_t plain = (int64_t)ctas_per_sm(threads, 64) * num_sms;
+  if (groups > 1024) return launch_bwd_one<block_norms_bwd_kernel<T, W, VEC, kWide, GATED, 1024, 0>>(a, plain, threads, 0, grid, st);
+  if constexpr (VEC) {
+    // four stages where they fit beside the SM's other CTAs, else two
+    const int per_sm = ctas_per_sm(threads, groups > 512 ? 64 : 112);
+    const int64_t most = (int64_t)per_sm * num_sms;
+    const int stage = a.slots * a.H * (int)sizeof(T), room = 220 * 1024 / per_sm - 1024;
+    if (4 * (stage + 8) <= room)
+      return groups > 512 ? launch_bwd_one<block_norms_bwd_kernel<T, W, VEC, 1, GATED, 1024, 4>>(a, most, threads, 4 * (stage + 8), grid, st)
+                          : launch_bwd_one<block_norms_bwd_kernel<T, W, VEC, 1, GATED, 512, 4>>(a, most, threads, 4 * (stage + 8), grid, st);
+    if (2 * (stage + 8) <= room)
+      return groups > 512 ? launch_bwd_one<block_norms_bwd_kernel<T, W, VEC, 1, GATED, 1024, 2>>(a, most, threads, 2 * (stage + 8), grid, st)
+                          : launch_bwd_one<block_norms_bwd_kernel<T, W, VEC, 1, GATED, 512, 2>>(a, most, threads, 2 * (stage + 8), grid, st);
+  }
+  return groups > 512 ? launch_bwd_one<block_norms_bwd_kernel<T, W, VEC, 1, GATED, 1024, 0>>(a, plain, threads, 0, grid, st)
+                      : launch_bwd_one<block_norms_bwd_kernel<T, W, VEC, 1, GATED, 512, 0>>(a, plain, threads, 0, grid, st);
+}
 template <typename T, typename W, bool VEC>
-static int launch_bwd(const BlockNormArgs& a, int grid, cudaStream_t st) {
-  return a.gate_kind == kGateNone ? launch_bwd_gate<T, W, VEC, false>(a, grid, st)
-                                  : launch_bwd_gate<T, W, VEC, true>(a, grid, st);
+static int launch_bwd(const BlockNormArgs& a, int num_sms, int* grid, cudaStream_t st) {
+  return a.gate_kind == kGateNone ? launch_bwd_gate<T, W, VEC, false>(a, num_sms, grid, st)
+                                  : launch_bwd_gate<T, W, VEC, true>(a, num_sms, grid, st);
 }
 
 // f(T, W, VEC) for the element type, the weights' type (that or fp32) and alignment.
@@ -485,9 +628,7 @@ int b200_block_norms_max_width() { return 4 * 1024 * 8; }
 // CTAs of the backward pass (rows of its partial sums) for T rows of H columns: what
 // fits on the SMs at 64 registers a thread.
 int b200_block_norms_bwd_grid(int64_t T, int H, int type, int num_sms) {
-  int per_sm = 1024 / bwd_threads(H, type);
-  per_sm = per_sm > 16 ? 16 : per_sm < 1 ? 1 : per_sm;
-  const int64_t most = (int64_t)per_sm * num_sms;
+  const int64_t most = (int64_t)ctas_per_sm(bwd_threads(H, type), 64) * num_sms;
   return (int)(T < most ? T : most);
 }
 
@@ -570,6 +711,7 @@ int b200_block_norms_bwd(const void* y, int64_t ldy, const void* delta, int64_t 
   a.gate_kind = gate_kind;
   a.scale = scale;
   a.offset_one = offset_one;
+  a.slots = 1 + (dy != nullptr) + 2 * (dh != nullptr) + (gate_kind == kGateElement);
   a.want_post = dpost != nullptr;
   a.want_pre = dpre != nullptr;
   a.want_gate = dgate != nullptr;
@@ -579,9 +721,9 @@ int b200_block_norms_bwd(const void* y, int64_t ldy, const void* delta, int64_t 
                    rows16(dx, 0) && rows16(ddelta, 0) && rows16(post, 0) && rows16(pre, 0) &&
                    (gate_kind == kGateRow ||
                     (rows16(gate, gate_kind == kGateElement ? ldg : 0) && (gate_kind != kGateElement || rows16(dgate, 0))));
-  const int grid = b200_block_norms_bwd_grid(T, H, type, num_sms);
+  int grid = 0;
   const int e = by_type(type, w_type, vec, [&](auto t, auto w, auto v) {
-    return launch_bwd<decltype(t), decltype(w), decltype(v)::value>(a, grid, st);
+    return launch_bwd<decltype(t), decltype(w), decltype(v)::value>(a, num_sms, &grid, st);
   });
   if (e) return e;
   ColSumArgs c = {};
