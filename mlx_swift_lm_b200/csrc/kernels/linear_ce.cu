@@ -3,6 +3,7 @@
 //   u = h . W^T,  z = cap > 0 ? cap * tanh(u / cap) : u          (T x V, never stored)
 //   d = log sum_{v != y} exp z_v - z_y,  loss = log(1 + exp d)
 //   G[t, v] = dloss_t * (p_v - [v = y]) * dz/du,  p_v = exp(z_v - z_y - loss)
+//   (dloss_t in dh and dW instead where it is the same for all t)
 //   dh = G . W,  dW = G^T . h
 //
 // The target's logit stands apart from the sum over the others, so a loss near
@@ -209,10 +210,20 @@ struct Walk {
   }
 };
 
-// Gradient of the loss with respect to the target's logit before the cap.
-__device__ __forceinline__ float target_grad(const Args& a, int row, float inv_n) {
+// What an upstream gradient multiplies: each row of G where every token has its own;
+// a common one (of a sum or mean) multiplies dh and dW in fp32 instead. The target's
+// entry, the largest of a row by far, is then 1 - p, and not a constant whose rounding
+// to bf16 would be the same for all rows and would not average out in dW.
+__device__ __forceinline__ float row_factor(const Args& a, int row) {
+  return a.dloss_stride ? a.dloss[a.dloss_stride * a.token[row]] : 1.f;
+}
+__device__ __forceinline__ float common_factor(const Args& a, int n) {
+  return (a.dloss_stride ? 1.f : *a.dloss) * (a.mean ? 1.f / (float)max(n, 1) : 1.f);
+}
+// The target's entry of G before it is rounded.
+__device__ __forceinline__ float target_grad(const Args& a, int row) {
   const float q = a.zt[row] * a.inv_cap;  // inv_cap 0: no cap
-  return expm1f(-a.loss[row]) * (1.f - q * q) * a.dloss[a.dloss_stride * a.token[row]] * (a.mean ? inv_n : 1.f);
+  return expm1f(-a.loss[row]) * (1.f - q * q) * row_factor(a, row);
 }
 
 // All pieces (the last may be shorter) and the final sum use the same parts.
@@ -361,7 +372,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int half = (warp - 4) >> 2, left = half * kHalfN;
     const bool first_thread = (threadIdx.x & 127) == 0;  // of the half
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const float inv_n = 1.f / (float)max(n, 1);
+    const float factor = OP == kDw ? common_factor(a, n) : 1.f;
     const uint32_t release = in_leader(bar_tempty);
     int tile = 0;
     bool dead = false;
@@ -381,8 +392,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           target = a.target[row] - (a.v0 + n0);  // its column in this tile, if within 0 .. 255
           if constexpr (OP == kGrad) {
             shift = (a.zt[row] + a.loss[row]) * kLog2e;
-            dl = a.dloss[a.dloss_stride * a.token[row]] * (a.mean ? inv_n : 1.f);
-            at_target = target_grad(a, row, inv_n);
+            dl = row_factor(a, row);
+            at_target = target_grad(a, row);
           }
         }
       }
@@ -485,7 +496,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               tc_wait_ld();
 #pragma unroll
               for (int j = 0; j < 32; j += 2)
-                o[(hh + j) / 2] = pack_bf16x2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]));
+                o[(hh + j) / 2] = pack_bf16x2(__uint_as_float(v[j]) * factor, __uint_as_float(v[j + 1]) * factor);
             }
           }
           if (OP != kGrad && empty) {
@@ -688,8 +699,8 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(MergeArgs a) {
   if (threadIdx.x == 0) *a.total = a.mean ? acc / (float)max(n, 1) : acc;
 }
 
-// dh[t] = sum over the contraction's parts of acc[.][place[t]] + e W[y], 0 for
-// ignored rows. e is what the target's entry of G lost when it was rounded to bf16:
+// dh[t] = (sum over the contraction's parts of acc[.][place[t]] + e W[y]) * factor, 0
+// for ignored rows. e is what the target's entry of G lost when it was rounded to bf16:
 // that entry alone is of the size of the whole row, the others are far below it, so
 // with it added back the rounding of G hardly shows in dh (measured against 64 bits:
 // 2.7e-3 -> 1.7e-3, the output's own rounding). A thread takes E columns of a row.
@@ -717,7 +728,7 @@ __global__ void __launch_bounds__(256) finish_dh_kernel(const FinishArgs a) {
   __nv_bfloat16* o = a.dh + (int64_t)t * a.g.K + c;
   float s[E] = {};
   if (p >= 0) {
-    const float g = target_grad(a.g, p, 1.f / (float)max(n, 1));
+    const float g = target_grad(a.g, p);
     const float e = g - bf2f(f2bf(g));
     const __nv_bfloat16* wr = a.w + (int64_t)max(a.g.target[p], 0) * a.ldw + c;
     const float* row = a.acc + (int64_t)p * a.lda + c;
@@ -738,6 +749,9 @@ __global__ void __launch_bounds__(256) finish_dh_kernel(const FinishArgs a) {
       s[0] = e * bf2f(*wr);
       for (int k = 0; k < parts; ++k) s[0] += row[k * part];
     }
+    const float factor = common_factor(a.g, n);
+#pragma unroll
+    for (int j = 0; j < E; ++j) s[j] *= factor;
   }
   if constexpr (E == 8)
     *reinterpret_cast<uint4*>(o) =

@@ -137,6 +137,17 @@ def test_a_row_does_not_depend_on_its_batch():
             assert torch.equal(yn, y[:n]) and torch.equal(hn, h[:n])
 
 
+@pytest.mark.parametrize("T,H,gate,kind", [(300, 512, "channel", 0), (300, 511, "row", 1), (40, 1024, "element", 2)])
+def test_each_gradient_by_itself(T, H, gate, kind):
+    ins, dy, dh = _inputs(T, H, torch.bfloat16, gate)
+    leaf = {k: t.detach().requires_grad_() for k, t in ins.items()}
+    all_of = dict(zip(leaf, torch.autograd.grad(ops.block_norms(**leaf), list(leaf.values()), [dy, dh])))
+    for name in ins:
+        one = {k: t.detach().requires_grad_(k == name) for k, t in ins.items()}
+        got, = torch.autograd.grad(ops.block_norms(**one), [one[name]], [dy, dh])
+        assert torch.equal(got, all_of[name]), name
+
+
 def test_bad_rows_stay_alone_and_repeat_bit_for_bit():
     ins, dy, dh = _inputs(50, 640, torch.bfloat16, "")
     ins["x"] = ins["x"].clone()

@@ -118,6 +118,38 @@ def test_directions(T, V, K, reduction, ignored, dh, dw):
     _check(T, V, K, reduction=reduction, ignored=ignored, dh=dh, dw=dw)
 
 
+@pytest.mark.parametrize("ignored", [0.0, 0.5, 0.95])
+def test_many_rows(ignored):
+    """More row tiles than one walk's column of them, and few scored rows among many."""
+    _check(4700, 600, 64, ignored=ignored)
+
+
+@pytest.mark.parametrize("T", [1, 7, 300])
+def test_one_upstream_gradient_for_all(T):
+    h, w, t = _inputs(T, 900, 128)
+    h, w = h.requires_grad_(), w.requires_grad_()
+    out = ops.linear_cross_entropy(h, w, t)
+    got = torch.autograd.grad(out, [h, w], torch.full((1,), 0.37, device=DEV).expand(T))
+    _, wh, ww = _expect(h.detach(), w.detach(), t, 0.0, "none", torch.full((T,), 0.37, device=DEV))
+    _within(got[0], wh, "dh")
+    _within(got[1], ww, "dW")
+
+
+def test_the_targets_rows_lose_little_to_rounding():
+    """With one upstream gradient and unsure rows the target's entries are near -1, whose rounding to bf16 does not
+    show: dW is off by its own rounding, not by a second one that all rows share (which 1 / 1365 would add)."""
+    h, w, t = _inputs(1365, 4000, 256, ignored=0.0, lean=0.0)
+    h, w = h.requires_grad_(), w.requires_grad_()
+    loss = ops.linear_cross_entropy(h, w, t, reduction="mean")
+    dh, dw = torch.autograd.grad(loss, [h, w])
+    hd, wd = h.detach().double(), w.detach().double()
+    G = torch.softmax(hd @ wd.t(), 1)
+    G[torch.arange(1365, device=DEV), t] -= 1
+    # rms of a bf16 rounding: at most 2^-8 / sqrt(3) of a value; twice that leaves no room for a second one of 2^-8
+    for got, want in ((dh, G @ wd / 1365), (dw, G.t() @ hd / 1365)):
+        assert (got.double() - want).norm() <= 1.25 * 2 ** -8 / 3 ** 0.5 * want.norm()
+
+
 @pytest.mark.parametrize("T,V,K", [(3, 300, 64), (140, 2000, 200), (64, 50257, 96)])
 def test_softcap(T, V, K):
     _check(T, V, K, cap=5.0)
