@@ -64,7 +64,15 @@ struct Args {
   int piece, pairs;      // kDh: columns of a whole piece and CTA pairs (choose_parts)
   int most_parts, first;  // kDh: parts the sums have room for; first piece stores, others add
   float cap, inv_cap;    // cap 0: none
+  float unbias;          // factor of the products' results (unbias_of)
 };
+
+// The tensor cores add each 16-deep step into the fp32 accumulator by truncation:
+// products of K terms come out too small by K / 16 steps of about 2^-26 (measured
+// against 64 bits on unit normal operands: 1.9e-7 at K = 256, 8.6e-7 at 1024, 3.8e-6
+// at 4096). Of a mean loss that would be the whole error, so the logits are scaled
+// back by it; what is left has either sign.
+static float unbias_of(int K) { return 1.f + (float)((K + 15) / 16) * (1.f / 67108864.f); }
 
 constexpr int kTileM = 256, kTileN = 256, kStages = 6;  // of a pair of CTAs
 constexpr int kRowsM = kTileM / 2, kRowsN = kTileN / 2;   // a CTA's share of either operand
@@ -372,6 +380,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int half = (warp - 4) >> 2, left = half * kHalfN;
     const bool first_thread = (threadIdx.x & 127) == 0;  // of the half
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    // logits as exponents of two, before the cap if there is one
+    const float to_log2 = a.cap > 0.f ? kLog2e : kLog2e * a.unbias, to_cap = a.inv_cap * a.unbias;
     const float factor = OP == kDw ? common_factor(a, n) : 1.f;
     const uint32_t release = in_leader(bar_tempty);
     int tile = 0;
@@ -410,7 +420,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           tc_wait_ld();
           if (a.cap > 0.f) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(a.cap * tanhf(__uint_as_float(v[j]) * a.inv_cap));
+            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(a.cap * tanhf(__uint_as_float(v[j]) * to_cap));
           }
           // columns past the vocabulary and the target's take no part
           if (c + 32 > cols || (unsigned)(target - c) < 32u) {
@@ -423,13 +433,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           for (int j = 1; j < 32; ++j) cm = fmaxf(cm, __uint_as_float(v[j]));
           const float m2 = fmaxf(mx, cm);
           if (m2 > -INFINITY) {
-            const float off = m2 * kLog2e;
-            sum = mx > -INFINITY ? sum * ex2(mx * kLog2e - off) : sum;  // 0, or NaN that stays
+            const float off = m2 * to_log2;
+            sum = mx > -INFINITY ? sum * ex2(mx * to_log2 - off) : sum;  // 0, or NaN that stays
             float s0 = 0.f, s1 = 0.f;
 #pragma unroll
             for (int j = 0; j < 32; j += 2) {
-              s0 += ex2(fmaf(__uint_as_float(v[j]), kLog2e, -off));
-              s1 += ex2(fmaf(__uint_as_float(v[j + 1]), kLog2e, -off));
+              s0 += ex2(fmaf(__uint_as_float(v[j]), to_log2, -off));
+              s1 += ex2(fmaf(__uint_as_float(v[j + 1]), to_log2, -off));
             }
             sum += s0 + s1;
             mx = m2;
@@ -442,6 +452,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) arrive_cluster(release + 8 * buf);
+        if (!(a.cap > 0.f)) mx *= a.unbias;
         // the right half's pair joins the left's; the buffers alternate between tiles, and the barrier
         // of the next tile is passed before one is written again
         float2* pairs_smem = reinterpret_cast<float2*>(smem + kStages * kStageBytes) + (tile & 1) * kRowsM;
@@ -474,11 +485,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 for (int e = 0; e < 2; ++e) {
                   float z = __uint_as_float(v[j + e]), slope = dl;
                   if (a.cap > 0.f) {
-                    const float q = tanh_fast(z * a.inv_cap);
+                    const float q = tanh_fast(z * to_cap);
                     z = a.cap * q;
                     slope *= 1.f - q * q;
                   }
-                  p[e] = ex2(fmaf(z, kLog2e, -shift)) * slope;
+                  p[e] = ex2(fmaf(z, to_log2, -shift)) * slope;
                   if (rel == j + e) p[e] = at_target;
                   if (row >= n || c + hh + j + e >= cols) p[e] = 0.f;
                 }
@@ -868,6 +879,7 @@ int b200_lce_forward(const void* h, int64_t ldh, const void* W, int64_t ldw, con
   a.nv = V;
   a.cap = p.cap;
   a.inv_cap = p.inv_cap;
+  a.unbias = unbias_of(K);
   CUtensorMap ta, tb;
   if (!make_tmap_2d(&ta, f.hc, T, Kp, Kp, kRowsM, 64, 2) || !make_tmap_2d(&tb, W, V, K, ldw, kRowsN, 64, 2)) return -1;
   if (int r = launch_gemm<kStats>(ta, tb, ta, a, tiles_of(T, kTileM) * tiles_of(V, kTileN), num_sms, st)) return r;
@@ -916,6 +928,7 @@ int b200_lce_backward(void* saved, const void* W, int64_t ldw, const float* dlos
   a.most_parts = most_parts(T, K, num_sms);
   a.cap = cap;
   a.inv_cap = cap > 0.f ? 1.f / cap : 0.f;
+  a.unbias = unbias_of(K);
   void* G = scratch;
   float* acc = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(scratch) + (int64_t)T * piece * 2);
   const int lda = acc_cols(K);
