@@ -208,8 +208,8 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
 struct Walk {
   int mt, nt, splits, total;
   __device__ __forceinline__ void at(int t, int& m, int& n, int& s) const {
-    s = t % splits;
-    t /= splits;
+    s = t / (mt * nt);
+    t -= s * mt * nt;
     const int per = kGroupM * nt;
     const int g = t / per, r = t - g * per;
     const int gm = min(kGroupM, mt - g * kGroupM);
