@@ -40,8 +40,8 @@ int b200_block_norms_bwd(const void* y, int64_t ldy, const void* delta, int64_t 
 
 // --- linear_ce.cu ---
 // What a forward pass leaves for its backward pass, in one buffer: the scored rows
-// [T, Kp] bf16, then their target logits and losses fp32 [T] each, then int32 count,
-// ticket, target [T], token [T], place [T].
+// [T, Kp] bf16, then their target logits, losses and logarithms of the sums of exp fp32
+// [T] each, then int32 count, ticket, target [T], token [T], place [T].
 int64_t b200_lce_saved_bytes(int T, int Kp);
 // Scratch of the forward pass: a (max, sum) pair per row and column tile.
 int64_t b200_lce_forward_bytes(int T, int V);

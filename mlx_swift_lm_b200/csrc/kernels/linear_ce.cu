@@ -2,7 +2,7 @@
 //
 //   u = h . W^T,  z = cap > 0 ? cap * tanh(u / cap) : u          (T x V, never stored)
 //   d = log sum_{v != y} exp z_v - z_y,  loss = log(1 + exp d)
-//   G[t, v] = dloss_t * (p_v - [v = y]) * dz/du,  p_v = exp(z_v - z_y - loss)
+//   G[t, v] = dloss_t * (p_v - [v = y]) * dz/du,  p_v = exp(z_v - lse), lse = log sum exp z
 //   (dloss_t in dh and dW instead where it is the same for all t)
 //   dh = G . W,  dW = G^T . h
 //
@@ -54,6 +54,7 @@ struct Args {
   const int* token;      // [T] the scored row's index in the batch
   const float* zt;       // [T] target logits (capped)
   const float* loss;     // [T] losses of the scored rows
+  const float* lse;      // [T] logarithms of their sums of exp
   const float* dloss;    // incoming gradient, element token * dloss_stride
   int64_t dloss_stride;
   int mean;              // dloss is of the mean: divide by n
@@ -304,6 +305,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     if (lane == 0) {
+      // both operands are read by several pairs and rounds (4096 rows: 15.9 ms a step; 16.2 with W
+      // evict-normal, 16.3 evict-first)
       const uint64_t pol = l2_policy_evict_last();
       int it = 0;
       bool ok = true;
@@ -401,7 +404,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (row < n) {
           target = a.target[row] - (a.v0 + n0);  // its column in this tile, if within 0 .. 255
           if constexpr (OP == kGrad) {
-            shift = (a.zt[row] + a.loss[row]) * kLog2e;
+            shift = a.lse[row] * kLog2e;
             dl = row_factor(a, row);
             at_target = target_grad(a, row);
           }
@@ -658,6 +661,7 @@ struct MergeArgs {
   const int *count, *token;
   const float* zt;
   float* row_loss;  // [T] by scored row
+  float* lse;       // [T] by scored row (not zt + loss: a target far below the others would leave none of its digits)
   float* loss;      // [T] by token
   float* total;     // [1] sum or mean, or null
   unsigned* ticket;
@@ -691,10 +695,11 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(MergeArgs a) {
   if (warp == 0 && row < n) {
     for (int i = 1; i < kMergeWarps; ++i) join(m, s, sh[i][lane].x, sh[i][lane].y);
     // s = 0 (a vocabulary of one): d = -inf, loss 0
-    const float d = m + logf(s) - a.zt[row];
-    const float l = d == -INFINITY ? 0.f : fmaxf(d, 0.f) + log1pf(expf(-fabsf(d)));
-    const float loss = d != d ? d : l;
+    const float zt = a.zt[row], others = m + logf(s), d = others - zt;
+    const float more = d == -INFINITY ? 0.f : log1pf(expf(-fabsf(d)));
+    const float loss = d != d ? d : fmaxf(d, 0.f) + more;
     a.row_loss[row] = loss;
+    a.lse[row] = d != d ? d : fmaxf(others, zt) + more;
     a.loss[a.token[row]] = loss;
   }
   if (a.total == nullptr) return;
@@ -793,9 +798,9 @@ using namespace b200::lce;
 extern "C" {
 
 // What a forward pass leaves for its backward pass, in one buffer of
-// b200_lce_saved_bytes: hc [T, Kp] bf16, then zt and row loss fp32 [T] each, then
+// b200_lce_saved_bytes: hc [T, Kp] bf16, then zt, row loss and lse fp32 [T] each, then
 // int32 count, ticket, target [T], token [T], place [T].
-int64_t b200_lce_saved_bytes(int T, int Kp) { return (int64_t)T * Kp * 2 + ((int64_t)5 * T + 2) * 4; }
+int64_t b200_lce_saved_bytes(int T, int Kp) { return (int64_t)T * Kp * 2 + ((int64_t)6 * T + 2) * 4; }
 
 // Scratch of the forward pass: a (max, sum) pair per row and column tile.
 int64_t b200_lce_forward_bytes(int T, int V) { return (int64_t)T * tiles_of(V, kTileN) * 8; }
@@ -817,13 +822,14 @@ int64_t b200_lce_backward_bytes(int T, int K, int piece, int want_dh, int num_sm
 
 struct Saved {
   uint8_t* hc;
-  float *zt, *loss;
+  float *zt, *loss, *lse;
   int *count, *target, *token, *place;
   Saved(void* p, int T, int Kp) {
     hc = reinterpret_cast<uint8_t*>(p);
     zt = reinterpret_cast<float*>(hc + (int64_t)T * Kp * 2);
     loss = zt + T;
-    count = reinterpret_cast<int*>(loss + T);
+    lse = loss + T;
+    count = reinterpret_cast<int*>(lse + T);
     target = count + 2;
     token = target + T;
     place = token + T;
@@ -889,6 +895,7 @@ int b200_lce_forward(const void* h, int64_t ldh, const void* W, int64_t ldw, con
   g.token = f.token;
   g.zt = f.zt;
   g.row_loss = f.loss;
+  g.lse = f.lse;
   g.loss = loss;
   g.total = total;
   g.ticket = p.ticket;
@@ -916,6 +923,7 @@ int b200_lce_backward(void* saved, const void* W, int64_t ldw, const float* dlos
   a.token = f.token;
   a.zt = f.zt;
   a.loss = f.loss;
+  a.lse = f.lse;
   a.dloss = dloss;
   a.dloss_stride = dloss_stride;
   a.mean = mean;

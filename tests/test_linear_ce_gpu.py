@@ -210,6 +210,27 @@ def test_a_bad_row_stays_alone_in_the_losses():
     assert torch.equal(out[rest], good[rest])
 
 
+@pytest.mark.parametrize("gap", [60.0, 1e4, 3e38])
+def test_a_target_far_below_the_others(gap):
+    """A head row of very low logits as the target: the others' probabilities keep their digits."""
+    h, w, t = _inputs(40, 500, 64, ignored=0.0, lean=0.0)
+    h[:, 0] = 1.0
+    w[7] = 0.0
+    w[7, 0] = -gap
+    t[:] = 7
+    a, b = h.detach().requires_grad_(), w.detach().requires_grad_()
+    dh, dw = torch.autograd.grad(ops.linear_cross_entropy(a, b, t, reduction="sum"), [a, b])
+    hd, wd = h.double(), w.double()
+    p = torch.softmax(hd @ wd.t(), 1)
+    p[:, 7] -= 1
+    rest = torch.arange(500, device=DEV) != 7
+    # bf16 G and the output's rounding: 2^-8 each of the terms
+    want = p.t() @ hd
+    assert ((dw.double() - want).abs() <= 2 * 2 ** -8 * (p.abs().t() @ hd.abs()) + 1e-6)[rest].all()
+    want = p[:, rest] @ wd[rest]
+    assert ((dh.double() - want)[:, 1:].abs() <= 3 * 2 ** -8 * (p[:, rest].abs() @ wd[rest].abs())[:, 1:] + 1e-6).all()
+
+
 def test_targets_out_of_range_are_reported():
     h, w, t = _inputs(10, 300, 64, ignored=0.0)
     good = ops.linear_cross_entropy(h, w, t)
