@@ -536,9 +536,11 @@ static inline int round32(int v) { return (v + 31) / 32 * 32; }
 
 // Groups of eight a thread, forward. Rows above 8192 columns need more than one for
 // each of 1024 threads. Below, one keeps a few rows' latency low and four leave room
-// for eight times the rows on an SM, whose loads then overlap the others' sums
-// (8192 x 4096 bf16: see kFewRows); both add in the same order. Unaligned rows are
-// dealt to the lanes by the thread count, so there the choice goes by the width alone.
+// for four times the rows on an SM, whose loads then overlap the others' sums; both add
+// in the same order. bf16 rows of 4096, one group against four: 64 rows 2.7 us against
+// 3.7, 592 rows 4.8 against 5.0, 1184 rows 8.3 against 6.5, 8192 rows 55 against 44 (6.1
+// TB/s). Unaligned rows are dealt to the lanes by the thread count, so there the choice
+// goes by the width alone.
 constexpr int kFewRows = 4;  // rows an SM
 template <typename T, typename W, bool VEC, bool GATED>
 static int launch_fwd_gate(const BlockNormArgs& a, int num_sms, cudaStream_t st) {
