@@ -150,6 +150,28 @@ def test_the_targets_rows_lose_little_to_rounding():
         assert (got.double() - want).norm() <= 1.25 * 2 ** -8 / 3 ** 0.5 * want.norm()
 
 
+@pytest.mark.parametrize("T,V,K", [(1, 257, 256), (2, 3, 100), (33, 9000, 72), (64, 300, 520)])
+def test_few_rows_keep_their_targets_entries(T, V, K):
+    """Up to 64 rows the targets' entries of G reach dW unrounded: what is left is dW's own rounding
+    (half a step) and that of other rows' entries in the same column."""
+    h, w, t = _inputs(T, V, K, ignored=0.0, lean=0.0)
+    t = t % max(1, V // 2)  # some rows share a target
+    h, w = h.requires_grad_(), w.requires_grad_()
+    weights = torch.rand(T, device=DEV) + 0.5
+    dw, = torch.autograd.grad(ops.linear_cross_entropy(h, w, t), [w], weights)
+    hd, wd = h.detach().double(), w.detach().double()
+    G = torch.softmax(hd @ wd.t(), 1)
+    G[torch.arange(T, device=DEV), t] -= 1
+    want = (G * weights[:, None].double()).t() @ hd
+    rows = torch.unique(t)
+    half_step = torch.finfo(torch.bfloat16).eps / 2
+    others = G.clone()
+    others[torch.arange(T, device=DEV), t] = 0
+    off = half_step * ((others.abs() * weights[:, None].double()).t() @ hd.abs())[rows]
+    limit = half_step * want[rows].abs() + off + 1e-6 * (G.abs().t() @ hd.abs())[rows]
+    assert ((dw.double() - want)[rows].abs() <= limit).all()
+
+
 @pytest.mark.parametrize("T,V,K", [(3, 300, 64), (140, 2000, 200), (64, 50257, 96)])
 def test_softcap(T, V, K):
     _check(T, V, K, cap=5.0)

@@ -121,6 +121,44 @@ def test_two_captured_steps_do_not_share_workspaces():
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_steps_leave_no_memory_behind():
+    leaves, w, t = _inputs()
+    dev = [v.to(DEV).requires_grad_() for v in leaves]
+    w, t = w.to(DEV), t.to(DEV)
+
+    def step():
+        loss = _step(*dev, w, t, 0.2, 9, 4, torch.bfloat16)
+        torch.autograd.grad(loss, dev)
+        _step(*dev, w, t, 0.2, 9, 4, torch.bfloat16)  # and a graph that is dropped
+
+    step()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for _ in range(20):
+        step()
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() == before
+
+
+def test_the_same_leaf_twice():
+    x = torch.randn(6, 32, device=DEV, requires_grad=True)
+    w = torch.ones(32, device=DEV, requires_grad=True)
+    y, h = ops.block_norms(x, x, w, w)
+    gx, gw = torch.autograd.grad(y.sum() + (h * h).sum(), [x, w])
+    xd, wd = x.detach().double().requires_grad_(), w.detach().double().requires_grad_()
+    rms = lambda v: v * (v.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * wd  # noqa: E731
+    yd = xd + rms(xd)
+    want = torch.autograd.grad(yd.sum() + rms(yd).square().sum(), [xd, wd])
+    assert torch.allclose(gx.double(), want[0], rtol=1e-4, atol=1e-4) and torch.allclose(gw.double(), want[1], rtol=1e-4, atol=1e-4)
+    a = torch.randn(6, 32, device=DEV)
+    b, c = a.clone(), a.clone()
+    y, _ = ops.block_norms(b, b, w.detach(), None, inplace=True)
+    assert torch.equal(y, ops.block_norms(a, c, w.detach(), None)[0])
+    z = ops.dropout(x, 0.5, 3, residual=x)
+    keep = ref.dropout_keep_ref(6, 32, 0.5, 3).to(DEV)
+    assert torch.equal(torch.autograd.grad(z.sum(), x)[0], 1 + 2.0 * keep)
+
+
 def test_gradients_are_taken_once():
     x = torch.randn(4, 32, device=DEV, requires_grad=True)
     w = torch.randn(40, 32, device=DEV).bfloat16()
