@@ -11,6 +11,7 @@
 // that whichever build of it Python loaded (release or checked) is the one called.
 // Checks run for any device; a call on CPU tensors returns None, and the Python
 // side answers it from the reference.
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -112,6 +113,22 @@ using Maybe = std::optional<Tensor>;
 Tensor opt(const Maybe& t) { return t.has_value() ? *t : Tensor(); }
 Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
 
+// A graph of the same leaf that was made on another stream and still lives holds the
+// leaf's gradient accumulation on that stream; the engine would make the captured
+// backward pass wait for it, which a capture cannot, and from its thread that ends the
+// process. The forward call of such a step is refused while it can be.
+void capturable(const char* what, std::initializer_list<Tensor> inputs) {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  for (const Tensor& t : inputs) {
+    if (!wants_grad(t) || !t.is_leaf() || !t.is_cuda()) continue;
+    const auto held = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (!held) continue;
+    const auto stream = held->stream();
+    TORCH_CHECK(!stream || *stream == c10::cuda::getCurrentCUDAStream(t.device().index()).unwrap(), what,
+                ": a graph of the same leaf, made on another stream, is still alive; drop its outputs before the capture");
+  }
+}
+
 void once(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, ": the gradient is not differentiable a second time");
 }
@@ -172,8 +189,10 @@ Maybe dropout(const Tensor& x, double p, uint64_t seed, uint64_t offset, const M
   if (!x.is_cuda()) return std::nullopt;
   TORCH_CHECK_VALUE((x.dim() ? x.size(-1) : 1) <= INT32_MAX, "dropout: rows of ", x.size(-1), " columns");
   const int64_t cut = (int64_t)(p * 65536 + 0.5);
-  if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(residual)))
+  if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(residual))) {
+    capturable("dropout", {x, residual});
     return Dropout::apply(x, maybe(residual), cut, (int64_t)seed, (int64_t)offset, maybe(off));
+  }
   return dropout_run(x, cut, seed, offset, off, residual);
 }
 
@@ -319,6 +338,7 @@ std::optional<std::pair<Tensor, Maybe>> block_norms(
   TORCH_CHECK_VALUE(H <= lib.b200_block_norms_max_width(), "block_norms: ", H, " columns, at most ",
                     lib.b200_block_norms_max_width());
   if (grad) {
+    capturable("block_norms", {x, delta, post, pre, gate});
     const auto out = BlockNorms::apply(x, delta, maybe(post), maybe(pre), maybe(gate), kind, eps, scale, offset_one, round_branch);
     return std::make_pair(out[0], out.size() > 1 ? Maybe(out[1]) : std::nullopt);
   }
@@ -423,6 +443,7 @@ Maybe linear_cross_entropy(const Tensor& h, const Tensor& w, const Tensor& targe
   const Tensor h2 = rows2d(h, K), t1 = targets.reshape(-1).contiguous();
   Tensor out;
   if (at::GradMode::is_enabled() && (h.requires_grad() || w.requires_grad())) {
+    capturable("linear_cross_entropy", {h, w});
     constexpr int64_t kTile = 256;  // pieces of the vocabulary are whole tiles
     const int64_t piece = std::min(std::max(min_piece, piece_bytes / (2 * T) / kTile * kTile), (V + kTile - 1) / kTile * kTile);
     out = LinearCe::apply(h2, w, t1, cap, ignore, reduction, piece);

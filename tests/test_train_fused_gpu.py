@@ -159,6 +159,31 @@ def test_the_same_leaf_twice():
     assert torch.equal(torch.autograd.grad(z.sum(), x)[0], 1 + 2.0 * keep)
 
 
+def test_a_capture_beside_a_living_eager_graph_is_refused():
+    x = torch.randn(6, 32, device=DEV, requires_grad=True)
+    w = torch.randn(40, 32, device=DEV).bfloat16()
+    hb = torch.randn(6, 32, device=DEV).bfloat16().requires_grad_()
+    t = torch.arange(6, device=DEV)
+    calls = [(x, lambda: ops.dropout(x, 0.5, 1)), (x, lambda: ops.block_norms(x, x, None, torch.ones(32, device=DEV))[1]),
+             (hb, lambda: ops.linear_cross_entropy(hb, w, t))]
+    for leaf, call in calls:
+        kept = call()  # an eager graph on the default stream
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="still alive"):
+            with torch.cuda.graph(g):
+                call()
+        want, = torch.autograd.grad(kept.sum(), leaf)
+        del kept
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got, = torch.autograd.grad(call().sum(), leaf)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
 def test_gradients_are_taken_once():
     x = torch.randn(4, 32, device=DEV, requires_grad=True)
     w = torch.randn(40, 32, device=DEV).bfloat16()
