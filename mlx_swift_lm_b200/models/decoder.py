@@ -522,7 +522,7 @@ class DecoderLM:
             if hook is not None and li > 0:
                 x, delta = hook(li - 1, x, self._post_norm(delta, post))
                 post = None
-            h = self._norm(x, delta, L.ln1, L.ln1_b, post)
+            h = self._norms(x, delta, L.ln1, L.ln1_b, post)
             post = None
             if L.block == "ffn":  # FFN-only layer (NemotronH "-" / "E")
                 delta = self._mlp(L, h)
@@ -538,7 +538,7 @@ class DecoderLM:
             post = L.post_attn_norm
             if L.block == "mixer":
                 continue
-            h = self._norm(x, delta, L.ln2, L.ln2_b, post)
+            h = self._norms(x, delta, L.ln2, L.ln2_b, post)
             delta = self._mlp(L, h)
             post = L.post_ffn_norm
         delta = self._post_norm(delta, post)
@@ -632,18 +632,24 @@ class DecoderLM:
         cfg = self.cfg
         return delta if post is None else ops.rmsnorm(delta, post, cfg.rms_norm_eps, cfg.norm_offset_one)
 
-    def _norm(self, x, delta, w, b=None, post=None):
+    def _norms(self, x, delta, w, b, post):
+        """:meth:`_norm` of a delta that first passes the previous block's output norm
+        `post` (or none). Both norms and the add are one launch, rounded where separate
+        ones round; a subclass with a :meth:`_norm` of its own gets the separate ones."""
+        if post is None or delta is None:
+            return self._norm(x, delta, w, b)
+        cfg = self.cfg
+        if (type(self)._norm is DecoderLM._norm and cfg.norm_kind != "layernorm" and delta.dtype == post.dtype == x.dtype
+                and (w is None or w.dtype == x.dtype)):
+            h = ops.block_norms(x, delta, post, w, cfg.rms_norm_eps, offset_one=cfg.norm_offset_one,
+                                round_branch=True, inplace=True)[1]
+            return x if h is None else h
+        return self._norm(x, self._post_norm(delta, post), w, b)
+
+    def _norm(self, x, delta, w, b=None):
         """x <- x + delta; the block's input norm (RMSNorm, or LayerNorm with bias).
-        `post`: the previous block's output norm, which delta passes first; both
-        norms and the add are one launch, rounded where separate ones round.
         Blocks without input norms (OLMo 2/3, EXAONE 4) get the residual stream itself."""
         cfg = self.cfg
-        if post is not None and delta is not None:
-            if cfg.norm_kind != "layernorm" and delta.dtype == post.dtype == x.dtype and (w is None or w.dtype == x.dtype):
-                h = ops.block_norms(x, delta, post, w, cfg.rms_norm_eps, offset_one=cfg.norm_offset_one,
-                                    round_branch=True, inplace=True)[1]
-                return x if h is None else h
-            delta = self._post_norm(delta, post)
         if w is None and not cfg.pre_norms:
             if delta is not None:
                 x.add_(delta)
@@ -785,7 +791,7 @@ class DecoderLM:
         x = ops.embedding(tokens.to(torch.int32), self.embed, cfg.embed_scale)
         delta = post = None
         for li, L in enumerate(self.layers):
-            h = self._norm(x, delta, L.ln1, L.ln1_b, post)
+            h = self._norms(x, delta, L.ln1, L.ln1_b, post)
             post = None
             if L.block == "ffn":
                 delta = self._mlp(L, h)
@@ -833,11 +839,11 @@ class DecoderLM:
             post = L.post_attn_norm
             if L.block == "mixer":
                 continue
-            h = self._norm(x, delta, L.ln2, L.ln2_b, post)
+            h = self._norms(x, delta, L.ln2, L.ln2_b, post)
             delta = self._mlp(L, h)
             post = L.post_ffn_norm
         cache.offset += Lq
-        h = self._norm(x, delta, self.norm, self.norm_b, post)
+        h = self._norms(x, delta, self.norm, self.norm_b, post)
         if return_hidden:
             return h
         return self._final_logits(h)
