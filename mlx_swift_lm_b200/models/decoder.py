@@ -632,6 +632,12 @@ class DecoderLM:
         cfg = self.cfg
         return delta if post is None else ops.rmsnorm(delta, post, cfg.rms_norm_eps, cfg.norm_offset_one)
 
+    @staticmethod
+    def _fuses_norms(x, delta, *weights) -> bool:
+        """Whether ops.block_norms takes these: the kernels' types, the same throughout
+        (float64 models on CPU run the separate norms)."""
+        return x.dtype in ops.BLOCK_NORMS_DTYPES and all(t is None or t.dtype == x.dtype for t in (delta, *weights))
+
     def _norms(self, x, delta, w, b, post):
         """:meth:`_norm` of a delta that first passes the previous block's output norm
         `post` (or none). Both norms and the add are one launch, rounded where separate
@@ -639,8 +645,7 @@ class DecoderLM:
         if post is None or delta is None:
             return self._norm(x, delta, w, b)
         cfg = self.cfg
-        if (type(self)._norm is DecoderLM._norm and cfg.norm_kind != "layernorm" and delta.dtype == post.dtype == x.dtype
-                and (w is None or w.dtype == x.dtype)):
+        if type(self)._norm is DecoderLM._norm and cfg.norm_kind != "layernorm" and self._fuses_norms(x, delta, post, w):
             h = ops.block_norms(x, delta, post, w, cfg.rms_norm_eps, offset_one=cfg.norm_offset_one,
                                 round_branch=True, inplace=True)[1]
             return x if h is None else h

@@ -262,15 +262,22 @@ class Gemma4LM(DecoderLM):
         m2 = ops.rmsnorm(e, L.g4_post_ffn2, eps)
         return (m1.float() + m2.float()).to(x.dtype)
 
+    def _add_branch(self, x, out, post, pre=None):
+        """(x + RMSNorm(out) * post, that normed with `pre`, or None without it)."""
+        eps = self.cfg.rms_norm_eps
+        if self._fuses_norms(x, out, post, pre):
+            return ops.block_norms(x, out, post, pre, eps, round_branch=True)
+        x = (x.float() + ops.rmsnorm(out, post, eps).float()).to(x.dtype)
+        return x, None if pre is None else ops.rmsnorm(x, pre, eps)
+
     def _block_tail(self, L, li, x, attn_out, ple):
         """Everything after attention: residual adds, FFN, per-layer input, scalar."""
-        eps = self.cfg.rms_norm_eps
-        x, h = ops.block_norms(x, attn_out, L.post_attn_norm, L.ln2, eps, round_branch=True)
-        x, _ = ops.block_norms(x, self._ffn(L, x, h), L.post_ffn_norm, None, eps, round_branch=True)
+        x, h = self._add_branch(x, attn_out, L.post_attn_norm, L.ln2)
+        x, _ = self._add_branch(x, self._ffn(L, x, h), L.post_ffn_norm)
         if ple is not None:
             gt = ops.gemm(x, L.ple_gate, epi="gelu_tanh")
             gt = (gt.float() * ple[:, li].float()).to(x.dtype)
-            x, _ = ops.block_norms(x, ops.gemm(gt, L.ple_proj), L.ple_norm, None, eps, round_branch=True)
+            x, _ = self._add_branch(x, ops.gemm(gt, L.ple_proj), L.ple_norm)
         return (x.float() * L.layer_scalar.float()).to(x.dtype)
 
     def _qkv_parts(self, L, li, h):

@@ -6,5 +6,6 @@ from .attention import decode_max_parts, paged_decode, paged_prefill, paged_sele
 from .drop import dropout  # noqa: F401
 from .linear import WORKSPACE, gemm, gemm_qkv_rope, row_roles  # noqa: F401
 from .loss import linear_cross_entropy  # noqa: F401
-from .norm import add_layernorm, add_rmsnorm, block_norms, embedding, qk_norm_rope_kv, rmsnorm, silu_mul, xielu  # noqa: F401
+from .norm import (BLOCK_NORMS_DTYPES, add_layernorm, add_rmsnorm, block_norms, embedding, qk_norm_rope_kv,  # noqa: F401
+                   rmsnorm, silu_mul, xielu)
 from .sampling import argmax, argmax_confidence, logprobs, process_logits, sample  # noqa: F401

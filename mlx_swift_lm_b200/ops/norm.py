@@ -57,6 +57,9 @@ def rmsnorm(x, w, eps, offset_one=False):
     return add_rmsnorm(x, None, w, eps, offset_one=offset_one)
 
 
+BLOCK_NORMS_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
 def block_norms(x: torch.Tensor, delta: torch.Tensor, post_w: torch.Tensor | None = None,
                 pre_w: torch.Tensor | None = None, eps: float = 1e-6, gate: torch.Tensor | None = None,
                 scale: float = 1.0, offset_one: bool = False, round_branch: bool = False, inplace: bool = False):
