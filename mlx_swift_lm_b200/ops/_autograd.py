@@ -18,11 +18,35 @@ _bound = False
 _lib.register_signatures({}, status_tags=("dropout", "block_norms", "linear_ce"))
 
 
+class _Unbuilt:
+    """Stands in for the module on CPU where nothing has been built: the oracles answer,
+    and refuse what they cannot compute."""
+
+    @staticmethod
+    def dropout(x, p, *rest):
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"dropout probability {p} is not in [0, 1]")
+
+    @staticmethod
+    def block_norms(x, delta, *rest):
+        if delta.shape != x.shape:
+            raise ValueError(f"block_norms: delta {tuple(delta.shape)} for x {tuple(x.shape)}")
+
+    @staticmethod
+    def linear_cross_entropy(h, w, targets, softcap, ignore_index, reduction, *rest):
+        if reduction not in ("none", "sum", "mean"):
+            raise ValueError(f"linear_cross_entropy: reduction '{reduction}'")
+
+
+def _path():
+    return glob.glob(os.path.join(os.path.dirname(_lib.LIB_PATH), "_b200torch*.so"))
+
+
 def module():
     """The module, loaded once. Calls on CPU tensors check their arguments and return None."""
     global _module
     if _module is None:
-        path = glob.glob(os.path.join(os.path.dirname(_lib.LIB_PATH), "_b200torch*.so"))
+        path = _path()
         if not path:
             raise _lib.KernelLibraryMissing("_b200torch is missing: build it with `python mlx_swift_lm_b200/_build.py`")
         spec = importlib.util.spec_from_file_location("_b200torch", path[0])
@@ -45,4 +69,6 @@ def cuda_module():
 
 
 def for_device(t):
-    return cuda_module() if t.is_cuda else module()
+    if t.is_cuda:
+        return cuda_module()
+    return module() if _module is not None or _path() else _Unbuilt
