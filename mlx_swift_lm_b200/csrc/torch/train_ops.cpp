@@ -343,6 +343,8 @@ std::optional<std::pair<Tensor, Maybe>> block_norms(
     return std::make_pair(out[0], out.size() > 1 ? Maybe(out[1]) : std::nullopt);
   }
   const auto out = norms_run(x, delta, post, pre, gate, {kind, eps, scale, offset_one, round_branch}, inplace ? x : Tensor(), false);
+  // a node that saved x before has to see that it changed (inference tensors have no counter)
+  if (inplace && !x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
   return std::make_pair(out[0], maybe(out[1]));
 }
 
