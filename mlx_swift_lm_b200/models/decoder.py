@@ -641,11 +641,14 @@ class DecoderLM:
     def _norms(self, x, delta, w, b, post):
         """:meth:`_norm` of a delta that first passes the previous block's output norm
         `post` (or none). Both norms and the add are one launch, rounded where separate
-        ones round; a subclass with a :meth:`_norm` of its own gets the separate ones."""
+        ones round; a subclass with a :meth:`_norm` of its own gets the separate ones, and
+        so does a forward pass that autograd records (the one launch writes into x)."""
         if post is None or delta is None:
             return self._norm(x, delta, w, b)
         cfg = self.cfg
-        if type(self)._norm is DecoderLM._norm and cfg.norm_kind != "layernorm" and self._fuses_norms(x, delta, post, w):
+        grads = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, delta, post, w))
+        if (type(self)._norm is DecoderLM._norm and cfg.norm_kind != "layernorm" and not grads
+                and self._fuses_norms(x, delta, post, w)):
             h = ops.block_norms(x, delta, post, w, cfg.rms_norm_eps, offset_one=cfg.norm_offset_one,
                                 round_branch=True, inplace=True)[1]
             return x if h is None else h
