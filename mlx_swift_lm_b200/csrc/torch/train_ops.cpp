@@ -210,6 +210,23 @@ Tensor gate_rows(const Tensor& gate, int64_t kind, int64_t H) {
 }
 Tensor packed(const Tensor& w) { return w.defined() ? w.contiguous() : w; }
 
+// An in-place call reads `t` ([rows, cols] with rows `ld` apart) while other CTAs write rows of
+// x. That is sound where t's elements are none of x's, or (aligned: one for each of x's) where
+// each is the very element of x that its thread writes, which reads it before.
+void inplace_reads(const char* what, const Tensor& x2, const Tensor& t, int64_t rows, int64_t cols, int64_t ld, bool aligned) {
+  if (!t.defined() || x2.numel() == 0 || rows == 0) return;
+  const int64_t xs = x2.element_size(), ts = t.element_size();
+  const int64_t xp = (int64_t)reinterpret_cast<uintptr_t>(x2.data_ptr()), tp = (int64_t)reinterpret_cast<uintptr_t>(t.data_ptr());
+  const int64_t width = x2.size(1) * xs, step = x2.stride(0) * xs;
+  if (tp >= xp + (x2.size(0) - 1) * step + width || tp + (rows - 1) * ld * ts + cols * ts <= xp) return;
+  if (aligned && tp == xp && (rows == 1 || ld * ts == step)) return;
+  if (x2.size(0) > 1 && (rows == 1 || ld * ts == step)) {  // beside x's columns in the rows of one buffer
+    const int64_t off = ((tp - xp) % step + step) % step;
+    if (off >= width && off + cols * ts <= step) return;
+  }
+  TORCH_CHECK_VALUE(false, "block_norms: inplace writes x, whose memory ", what, " shares");
+}
+
 // {y, h, r1, r2}; y is written into `into` when given. r1 / r2 (the reciprocal RMS of
 // delta and y) are kept for the backward pass with `save`.
 std::array<Tensor, 4> norms_run(const Tensor& x, const Tensor& delta, const Tensor& post, const Tensor& pre, const Tensor& gate,
@@ -332,6 +349,15 @@ std::optional<std::pair<Tensor, Maybe>> block_norms(
     const Tensor rows = x.view({-1, H});
     TORCH_CHECK_VALUE(x.numel() == 0 || ((H == 1 || rows.stride(1) == 1) && (rows.size(0) == 1 || rows.stride(0) >= H)),
                       "block_norms: inplace needs rows of neighbouring columns that do not overlap");
+    if (x.numel()) {
+      const int64_t T = rows.size(0);
+      const Tensor d2 = rows2d(delta, H), g = gate_rows(gate, kind, H);
+      inplace_reads("delta", rows, d2, T, H, d2.stride(0), true);
+      inplace_reads("post_w", rows, packed(post), 1, H, H, false);
+      inplace_reads("pre_w", rows, packed(pre), 1, H, H, false);
+      if (kind == kElement) inplace_reads("the gate", rows, g, T, H, g.stride(0), true);
+      else inplace_reads("the gate", rows, g, 1, kind == kChannel ? H : T, 0, false);
+    }
   }
   if (!x.is_cuda()) return std::nullopt;
   if (!lib.bound) throw KernelFailure("the kernel library is not loaded");

@@ -75,7 +75,8 @@ def block_norms(x: torch.Tensor, delta: torch.Tensor, post_w: torch.Tensor | Non
     `offset_one`: the weights are stored minus one. `round_branch`: u is rounded
     to x's dtype before the gate, as a separate norm and add would (bit-equal to
     ``add_rmsnorm(x, rmsnorm(delta, post_w), pre_w)``). `inplace`: y is written
-    into x (no gradients).
+    into x (no gradients; of the other inputs' memory x may share only delta's or an
+    element gate's, and those element by element).
     """
     out = _autograd.for_device(x).block_norms(x, delta, post_w, pre_w, eps, gate, scale, offset_one, round_branch,
                                               inplace)
