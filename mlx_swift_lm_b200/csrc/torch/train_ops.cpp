@@ -103,9 +103,23 @@ Tensor empty(const Tensor& like, at::IntArrayRef shape, at::ScalarType type) {
   return at::empty(shape, like.options().dtype(type).requires_grad(false));
 }
 Tensor packed_like(const Tensor& t) { return at::empty(t.sizes(), t.options().requires_grad(false)); }
+// What a kernel reads or writes has memory: fake tensors and wrappers of other tensors have
+// none, and null would be their address.
+bool has_memory(const Tensor& t) {
+  return t.has_storage() && t.storage().unsafeGetStorageImpl()->_mutable_data_ptr_no_checks().get() != nullptr;
+}
+void in_memory(const Tensor& t) {
+  TORCH_CHECK_TYPE(!t.defined() || t.numel() == 0 || has_memory(t),
+                   "a training operator on a tensor without memory (a fake tensor or a wrapper)");
+}
 template <typename T = void>
 T* ptr(const Tensor& t) {
+  in_memory(t);
   return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr;
+}
+// Inputs that the kernels can answer for.
+void computable(std::initializer_list<Tensor> inputs) {
+  for (const Tensor& t : inputs) in_memory(t);
 }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 // autograd's argument lists hold no undefined tensors
@@ -142,7 +156,7 @@ Tensor dropout_run(const Tensor& x, int64_t cut, uint64_t seed, uint64_t offset,
   const int64_t K = x.dim() ? x.size(-1) : 1;
   const Tensor x2 = rows2d(x, K), r2 = residual.defined() ? rows2d(residual, K) : residual;
   const Launch on(x);
-  check(lib.b200_dropout(x2.data_ptr(), x2.stride(0), ptr(r2), r2.defined() ? r2.stride(0) : 0, y.data_ptr(), K, x2.size(0),
+  check(lib.b200_dropout(ptr(x2), x2.stride(0), ptr(r2), r2.defined() ? r2.stride(0) : 0, ptr(y), K, x2.size(0),
                          (int)K, elem_code(x, "dropout"), seed, offset, ptr<int64_t>(offset_t), (int)cut,
                          (float)(65536.0 / (65536 - cut)), num_sms(x.device()), on.stream),
         "dropout");
@@ -187,6 +201,7 @@ Maybe dropout(const Tensor& x, double p, uint64_t seed, uint64_t offset, const M
     same_device("dropout", x, off);
   }
   if (!x.is_cuda()) return std::nullopt;
+  computable({x, residual, off});
   TORCH_CHECK_VALUE((x.dim() ? x.size(-1) : 1) <= INT32_MAX, "dropout: rows of ", x.size(-1), " columns");
   const int64_t cut = (int64_t)(p * 65536 + 0.5);
   if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(residual))) {
@@ -214,9 +229,9 @@ Tensor packed(const Tensor& w) { return w.defined() ? w.contiguous() : w; }
 // x. That is sound where t's elements are none of x's, or (aligned: one for each of x's) where
 // each is the very element of x that its thread writes, which reads it before.
 void inplace_reads(const char* what, const Tensor& x2, const Tensor& t, int64_t rows, int64_t cols, int64_t ld, bool aligned) {
-  if (!t.defined() || x2.numel() == 0 || rows == 0) return;
+  if (!t.defined() || x2.numel() == 0 || rows == 0 || !has_memory(x2) || !has_memory(t)) return;
   const int64_t xs = x2.element_size(), ts = t.element_size();
-  const int64_t xp = (int64_t)reinterpret_cast<uintptr_t>(x2.data_ptr()), tp = (int64_t)reinterpret_cast<uintptr_t>(t.data_ptr());
+  const int64_t xp = (int64_t)reinterpret_cast<uintptr_t>(ptr(x2)), tp = (int64_t)reinterpret_cast<uintptr_t>(t.data_ptr());
   const int64_t width = x2.size(1) * xs, step = x2.stride(0) * xs;
   if (tp >= xp + (x2.size(0) - 1) * step + width || tp + (rows - 1) * ld * ts + cols * ts <= xp) return;
   if (aligned && tp == xp && (rows == 1 || ld * ts == step)) return;
@@ -243,9 +258,9 @@ std::array<Tensor, 4> norms_run(const Tensor& x, const Tensor& delta, const Tens
     const Tensor pw = packed(post), qw = packed(pre), g = gate_rows(gate, c.kind, H);
     const Tensor& w = pw.defined() ? pw : qw;
     const Launch on(x);
-    check(lib.b200_block_norms(x2.data_ptr(), x2.stride(0), d2.data_ptr(), d2.stride(0), ptr(pw), ptr(qw),
+    check(lib.b200_block_norms(ptr(x2), x2.stride(0), ptr(d2), d2.stride(0), ptr(pw), ptr(qw),
                                elem_code(w.defined() ? w : x, "block_norms weight"), ptr(g), c.kind == kElement ? g.stride(0) : 0,
-                               (int)c.kind, y2.data_ptr(), y2.stride(0), ptr(h), H, ptr<float>(r1), ptr<float>(r2), T, (int)H,
+                               (int)c.kind, ptr(y2), y2.stride(0), ptr(h), H, ptr<float>(r1), ptr<float>(r2), T, (int)H,
                                elem_code(x, "block_norms"), (float)c.eps, (float)c.scale, c.offset_one, c.round_branch,
                                num_sms(x.device()), on.stream),
           "block_norms");
@@ -297,7 +312,7 @@ struct BlockNorms : torch::autograd::Function<BlockNorms> {
     const Launch on(y);
     Tensor part;
     if (parts) part = empty(y, {(int64_t)parts * lib.b200_block_norms_bwd_grid(T, (int)H, type, sms) * H}, at::kFloat);
-    check(lib.b200_block_norms_bwd(y2.data_ptr(), y2.stride(0), d2.data_ptr(), d2.stride(0), ptr(pw), ptr(qw),
+    check(lib.b200_block_norms_bwd(ptr(y2), y2.stride(0), ptr(d2), d2.stride(0), ptr(pw), ptr(qw),
                                    elem_code(w.defined() ? w : y, "block_norms weight"), ptr(g),
                                    kind == kElement ? g.stride(0) : 0, (int)kind, ptr<float>(r1), ptr<float>(r2), ptr(dy2),
                                    dy2.defined() ? dy2.stride(0) : 0, ptr(dh2), dh2.defined() ? dh2.stride(0) : 0, ptr(dx),
@@ -360,6 +375,7 @@ std::optional<std::pair<Tensor, Maybe>> block_norms(
     }
   }
   if (!x.is_cuda()) return std::nullopt;
+  computable({x, delta, post, pre, gate});
   if (!lib.bound) throw KernelFailure("the kernel library is not loaded");
   TORCH_CHECK_VALUE(H <= lib.b200_block_norms_max_width(), "block_norms: ", H, " columns, at most ",
                     lib.b200_block_norms_max_width());
@@ -381,7 +397,7 @@ enum Reduction { kEach = 0, kSum = 1, kMean = 2 };
 // copy in padded rows.
 Tensor aligned_head(const Tensor& w) {
   const int64_t V = w.size(0), K = w.size(1);
-  if ((K == 1 || w.stride(1) == 1) && w.stride(0) % 8 == 0 && w.stride(0) >= K && (reinterpret_cast<uintptr_t>(w.data_ptr()) & 15) == 0)
+  if ((K == 1 || w.stride(1) == 1) && w.stride(0) % 8 == 0 && w.stride(0) >= K && (reinterpret_cast<uintptr_t>(ptr(w)) & 15) == 0)
     return w.detach();
   Tensor out = empty(w, {V, (K + 7) / 8 * 8}, at::kBFloat16).narrow(1, 0, K);
   out.copy_(w.detach());
@@ -400,8 +416,8 @@ CeOut ce_forward(const Tensor& h2, const Tensor& w_, const Tensor& targets, doub
   const Tensor loss = empty(h2, {T}, at::kFloat);
   Tensor total;
   if (reduction != kEach) total = empty(h2, {}, at::kFloat);
-  check(lib.b200_lce_forward(h2.data_ptr(), h2.stride(0), w.data_ptr(), w.stride(0), ptr<int64_t>(targets), ignore, (int)T,
-                             (int)V, (int)K, (int)Kp, (float)cap, saved.data_ptr(), part.data_ptr(), ptr<float>(loss),
+  check(lib.b200_lce_forward(ptr(h2), h2.stride(0), ptr(w), w.stride(0), ptr<int64_t>(targets), ignore, (int)T,
+                             (int)V, (int)K, (int)Kp, (float)cap, ptr(saved), ptr(part), ptr<float>(loss),
                              ptr<float>(total), reduction == kMean, num_sms(h2.device()), on.stream),
         "linear_cross_entropy");
   return {total.defined() ? total : loss, saved};
@@ -433,9 +449,9 @@ struct LinearCe : torch::autograd::Function<LinearCe> {
       dw = empty(w, {V, Kp}, at::kBFloat16);
       if (Kp != K) dw = dw.narrow(1, 0, K);
     }
-    check(lib.b200_lce_backward(saved.data_ptr(), w.data_ptr(), w.stride(0), ptr<float>(g),
+    check(lib.b200_lce_backward(ptr(saved), ptr(w), w.stride(0), ptr<float>(g),
                                 T > 1 && g.numel() == T ? g.stride(0) : 0, call[2] == kMean, (int)T, (int)V, (int)K, (int)Kp,
-                                (float)ctx->saved_data["cap"].toDouble(), (int)piece, scratch.data_ptr(), ptr(dh), ptr(dw), Kp,
+                                (float)ctx->saved_data["cap"].toDouble(), (int)piece, ptr(scratch), ptr(dh), ptr(dw), Kp,
                                 sms, on.stream),
           "linear_cross_entropy backward");
     return {dh, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
@@ -459,6 +475,7 @@ Maybe linear_cross_entropy(const Tensor& h, const Tensor& w, const Tensor& targe
   if (!h.is_cuda()) return std::nullopt;
   TORCH_CHECK_TYPE(h.scalar_type() == at::kBFloat16, "linear_cross_entropy: ", h.scalar_type(),
                    "; the CUDA kernels take bfloat16");
+  computable({h, w, targets});
   const int64_t T = targets.numel(), K = w.size(1), V = w.size(0);
   constexpr int64_t kMost = INT32_MAX - 65536;  // tile counts and coordinates are 32-bit
   TORCH_CHECK_VALUE(T <= kMost && V <= kMost && K <= kMost, "linear_cross_entropy: ", T, " rows, ", V, " x ", K, " head");
