@@ -117,9 +117,13 @@ T* ptr(const Tensor& t) {
   in_memory(t);
   return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr;
 }
-// Inputs that the kernels can answer for.
-void computable(std::initializer_list<Tensor> inputs) {
-  for (const Tensor& t : inputs) in_memory(t);
+// Inputs that the kernels can answer for: in memory, and without forward-mode tangents,
+// which a kernel would drop.
+void computable(const char* what, std::initializer_list<Tensor> inputs) {
+  for (const Tensor& t : inputs) {
+    in_memory(t);
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), what, ": forward-mode derivatives on CUDA");
+  }
 }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 // autograd's argument lists hold no undefined tensors
@@ -143,8 +147,10 @@ void capturable(const char* what, std::initializer_list<Tensor> inputs) {
   }
 }
 
-void once(const char* what) {
+// A backward pass's incoming gradients.
+void once(const char* what, const variable_list& grads) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, ": the gradient is not differentiable a second time");
+  for (const Tensor& g : grads) computable(what, {g});
 }
 
 // ------------------------------------------------------------------ dropout
@@ -174,7 +180,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
     return dropout_run(x, cut, (uint64_t)seed, (uint64_t)offset, off, residual);
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    once("dropout");
+    once("dropout", grads);
     const auto call = ctx->saved_data["call"].toIntVector();
     const auto off = ctx->saved_data.find("offset");
     Tensor dx, dr;
@@ -201,7 +207,7 @@ Maybe dropout(const Tensor& x, double p, uint64_t seed, uint64_t offset, const M
     same_device("dropout", x, off);
   }
   if (!x.is_cuda()) return std::nullopt;
-  computable({x, residual, off});
+  computable("dropout", {x, residual, off});
   TORCH_CHECK_VALUE((x.dim() ? x.size(-1) : 1) <= INT32_MAX, "dropout: rows of ", x.size(-1), " columns");
   const int64_t cut = (int64_t)(p * 65536 + 0.5);
   if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(residual))) {
@@ -282,7 +288,7 @@ struct BlockNorms : torch::autograd::Function<BlockNorms> {
     return {y};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    once("block_norms");
+    once("block_norms", grads);
     const auto saved = ctx->get_saved_variables();
     const Tensor &y = saved[0], &delta = saved[1], &post = saved[2], &pre = saved[3], &gate = saved[4], &r1 = saved[5],
                  &r2 = saved[6];
@@ -375,7 +381,7 @@ std::optional<std::pair<Tensor, Maybe>> block_norms(
     }
   }
   if (!x.is_cuda()) return std::nullopt;
-  computable({x, delta, post, pre, gate});
+  computable("block_norms", {x, delta, post, pre, gate});
   if (!lib.bound) throw KernelFailure("the kernel library is not loaded");
   TORCH_CHECK_VALUE(H <= lib.b200_block_norms_max_width(), "block_norms: ", H, " columns, at most ",
                     lib.b200_block_norms_max_width());
@@ -434,7 +440,7 @@ struct LinearCe : torch::autograd::Function<LinearCe> {
     return r.out;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    once("linear_cross_entropy");
+    once("linear_cross_entropy", grads);
     const auto kept = ctx->get_saved_variables();
     const Tensor &w_ = kept[0], &saved = kept[1];
     const auto call = ctx->saved_data["call"].toIntVector();
@@ -475,7 +481,7 @@ Maybe linear_cross_entropy(const Tensor& h, const Tensor& w, const Tensor& targe
   if (!h.is_cuda()) return std::nullopt;
   TORCH_CHECK_TYPE(h.scalar_type() == at::kBFloat16, "linear_cross_entropy: ", h.scalar_type(),
                    "; the CUDA kernels take bfloat16");
-  computable({h, w, targets});
+  computable("linear_cross_entropy", {h, w, targets});
   const int64_t T = targets.numel(), K = w.size(1), V = w.size(0);
   constexpr int64_t kMost = INT32_MAX - 65536;  // tile counts and coordinates are 32-bit
   TORCH_CHECK_VALUE(T <= kMost && V <= kMost && K <= kMost, "linear_cross_entropy: ", T, " rows, ", V, " x ", K, " head");
@@ -512,6 +518,8 @@ PYBIND11_MODULE(_b200torch, m) {
         PyErr_SetString(error->ptr(), e.what());
       } catch (const c10::ValueError& e) {
         PyErr_SetString(PyExc_ValueError, e.what_without_backtrace());
+      } catch (const c10::NotImplementedError& e) {
+        PyErr_SetString(PyExc_NotImplementedError, e.what_without_backtrace());
       } catch (const c10::TypeError& e) {
         PyErr_SetString(PyExc_TypeError, e.what_without_backtrace());
       }
