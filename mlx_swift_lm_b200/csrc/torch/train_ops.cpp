@@ -11,6 +11,7 @@
 // that whichever build of it Python loaded (release or checked) is the one called.
 // Checks run for any device; a call on CPU tensors returns None, and the Python
 // side answers it from the reference.
+#include <ATen/TracerMode.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -118,8 +119,10 @@ T* ptr(const Tensor& t) {
   return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr;
 }
 // Inputs that the kernels can answer for: in memory, and without forward-mode tangents,
-// which a kernel would drop.
+// which a kernel would drop. Nor is the call traced: a trace would hold the empty outputs and
+// not the launch.
 void computable(const char* what, std::initializer_list<Tensor> inputs) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!at::tracer::impl::is_dispatch_enabled(), what, ": torch.jit.trace on CUDA");
   for (const Tensor& t : inputs) {
     in_memory(t);
     TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), what, ": forward-mode derivatives on CUDA");

@@ -48,3 +48,11 @@ def test_function_transforms(which):
     for run in (lambda: torch.func.jvp(call, (x,), (torch.ones_like(x),)), lambda: torch.func.vmap(call)(x[None])):
         with pytest.raises((RuntimeError, TypeError, ValueError)):
             run()
+
+
+@pytest.mark.parametrize("which", [0, 2, 8])
+def test_traces(which):
+    x, call = _calls()[which]
+    with pytest.raises(NotImplementedError, match="jit.trace"):
+        torch.jit.trace(call, x)
+    call(x)
