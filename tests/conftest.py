@@ -1,5 +1,8 @@
+import functools
+import gc
 import os
 import sys
+import time
 
 import pytest
 
@@ -23,3 +26,28 @@ def pytest_collection_modifyitems(config, items):
     for it in items:
         if "gpu" in it.keywords:
             it.add_marker(skip)
+
+
+def settled(read):
+    """`read` of the allocator's count, once what nothing uses any more is gone: objects that wait for the
+    garbage collector, and what a thread of the autograd engine still holds. That thread wakes the caller
+    of a backward pass before it drops its own reference to the pass and the gradients in it, and where the
+    caller takes its processor the reference outlives the call by milliseconds."""
+
+    @functools.wraps(read)
+    def call(*args, **kw):
+        time.sleep(0.02)
+        gc.collect()
+        return read(*args, **kw)
+
+    return call
+
+
+@pytest.fixture(autouse=True)
+def _settled_allocator(request):
+    """Tests that name torch.cuda.memory_allocated read it settled."""
+    if "memory_allocated" in getattr(getattr(request.function, "__code__", None), "co_names", ()):
+        import torch
+
+        patch = request.getfixturevalue("monkeypatch")
+        patch.setattr(torch.cuda, "memory_allocated", settled(torch.cuda.memory_allocated))
