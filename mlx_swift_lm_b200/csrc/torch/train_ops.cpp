@@ -19,6 +19,8 @@
 
 #include <atomic>
 #include <optional>
+#include <unordered_set>
+#include <vector>
 
 #include "b200_train.h"
 
@@ -134,19 +136,33 @@ using Maybe = std::optional<Tensor>;
 Tensor opt(const Maybe& t) { return t.has_value() ? *t : Tensor(); }
 Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
 
-// A graph of the same leaf that was made on another stream and still lives holds the
-// leaf's gradient accumulation on that stream; the engine would make the captured
-// backward pass wait for it, which a capture cannot, and from its thread that ends the
-// process. The forward call of such a step is refused while it can be.
+// A node of the inputs' graph that was made on another stream, outside the capture, and still
+// lives: a leaf's accumulation that an eager graph keeps, or an eager part of this graph. The
+// engine would make the captured backward pass wait for its stream, which a capture cannot, and
+// from its thread that ends the process. The forward call of such a step is refused while it
+// can be.
 void capturable(const char* what, std::initializer_list<Tensor> inputs) {
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
-  for (const Tensor& t : inputs) {
-    if (!wants_grad(t) || !t.is_leaf() || !t.is_cuda()) continue;
-    const auto held = torch::autograd::impl::try_get_grad_accumulator(t);
-    if (!held) continue;
-    const auto stream = held->stream();
-    TORCH_CHECK(!stream || *stream == c10::cuda::getCurrentCUDAStream(t.device().index()).unwrap(), what,
-                ": a graph of the same leaf, made on another stream, is still alive; drop its outputs before the capture");
+  std::vector<std::shared_ptr<torch::autograd::Node>> todo;
+  for (const Tensor& t : inputs)
+    if (wants_grad(t) && t.is_cuda())
+      todo.push_back(t.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(t) : t.grad_fn());
+  std::unordered_set<const torch::autograd::Node*> seen;
+  while (!todo.empty()) {
+    const auto node = std::move(todo.back());
+    todo.pop_back();
+    if (!node || !seen.insert(node.get()).second) continue;
+    const auto stream = node->stream();
+    if (stream && stream->device_type() == c10::DeviceType::CUDA) {
+      const c10::cuda::CUDAStream made(*stream);
+      cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+      if (made != c10::cuda::getCurrentCUDAStream(made.device_index()) && made.stream() != nullptr &&
+          cudaStreamIsCapturing(made.stream(), &status) != cudaSuccess)
+        status = cudaStreamCaptureStatusNone, cudaGetLastError();
+      TORCH_CHECK(made == c10::cuda::getCurrentCUDAStream(made.device_index()) || status == cudaStreamCaptureStatusActive, what,
+                  ": a graph of the same leaf, made on another stream, is still alive; drop its outputs before the capture");
+    }
+    for (const auto& edge : node->next_edges()) todo.push_back(edge.function);
   }
 }
 
