@@ -195,8 +195,11 @@ __device__ __forceinline__ int choose_parts(int tiles, int kb, int pairs, int mo
   return (int)(__reduce_min_sync(0xffffffffu, best) % kMostParts) + 1;
 }
 
-// 1 - 2 / (1 + e^2x): off by at most 2^-22 of one, which is enough where the result is
-// rounded to bf16 (the losses take tanhf); 5 instructions for about 20.
+// 1 - 2 / (1 + e^2x): off by at most 2^-22 of one; 5 instructions for tanhf's 20 or so. The cap
+// multiplies that error in the exponent of G's entries, which are rounded to bf16 (2^-8 at
+// most): up to kFastTanhCap it stays below 2^-14 of an entry. Larger caps and the losses take
+// tanhf, whose error is relative.
+constexpr float kFastTanhCap = 256.f;
 __device__ __forceinline__ float tanh_fast(float x) {
   return 1.f - __fdividef(2.f, 1.f + ex2(2.f * kLog2e * x));
 }
@@ -518,16 +521,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               tmem_ld32(acc + c + hh, v);
               tc_wait_ld();
               const int rel = target - (c + hh);
+              if (a.cap > kFastTanhCap) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(tanhf(__uint_as_float(v[j]) * to_cap));
+              } else if (a.cap > 0.f) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(tanh_fast(__uint_as_float(v[j]) * to_cap));
+              }
 #pragma unroll
               for (int j = 0; j < 32; j += 2) {
                 float p[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                   float z = __uint_as_float(v[j + e]), slope = dl;
-                  if (a.cap > 0.f) {
-                    const float q = tanh_fast(z * to_cap);
-                    z = a.cap * q;
-                    slope *= 1.f - q * q;
+                  if (a.cap > 0.f) {  // z is the tanh
+                    slope *= 1.f - z * z;
+                    z *= a.cap;
                   }
                   p[e] = ex2(fmaf(z, to_log2, -shift)) * slope;
                   if (rel == j + e) p[e] = at_target;
