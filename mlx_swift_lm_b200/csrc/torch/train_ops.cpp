@@ -494,7 +494,9 @@ Maybe linear_cross_entropy(const Tensor& h, const Tensor& w, const Tensor& targe
   TORCH_CHECK_TYPE(targets.scalar_type() == at::kLong, "linear_cross_entropy: targets ", targets.scalar_type(), ", int64 needed");
   TORCH_CHECK_TYPE(h.scalar_type() == w.scalar_type() && h.is_floating_point(), "linear_cross_entropy: hidden rows ",
                    h.scalar_type(), ", head ", w.scalar_type());
-  TORCH_CHECK_VALUE(cap >= 0.0 && cap < INFINITY, "linear_cross_entropy: softcap ", cap);
+  // the kernels hold it and its reciprocal in 32 bits: neither may round to 0 (no cap) or inf
+  TORCH_CHECK_VALUE(cap == 0.0 || (cap >= 0x1p-126 && cap <= 0x1p126), "linear_cross_entropy: softcap ", cap,
+                    ", 0 or a value from 2^-126 to 2^126 needed");
   same_device("linear_cross_entropy", h, w);
   same_device("linear_cross_entropy", h, targets);
   if (!h.is_cuda()) return std::nullopt;

@@ -25,7 +25,7 @@ def linear_cross_entropy(h: torch.Tensor, w: torch.Tensor, targets: torch.Tensor
     forming them: fp32 losses, differentiable in h and w.
 
     h [..., K] and w [V, K] (bf16 on CUDA), targets [...] int64. `softcap` c > 0
-    caps the logits as c tanh(z / c). Positions whose target is `ignore_index`
+    (2^-126 to 2^126) caps the logits as c tanh(z / c). Positions whose target is `ignore_index`
     have loss 0, take no part in any gradient and cost nothing (only the others
     are computed). `reduction`: "none" (a loss per position), "sum", or "mean"
     over the scored positions (0 where there are none). Any other target outside

@@ -31,3 +31,24 @@ def test_gradients_of_logits_far_below_the_cap(T, V, K, cap):
         # G's entries are off by their bf16 rounding and the exponent's error (2^-14 of the fast tanh and ez), the
         # outputs by theirs: 2^-8 each at most, in norm
         assert (a.double() - b).norm() <= (2 * 2 ** -8 + 2 ** -13 + 2 * ez.amax()) * b.norm()
+
+
+@pytest.mark.parametrize("cap", [2.0 ** 126, 2.0 ** -126])
+def test_the_ends_of_the_range(cap):
+    g = torch.Generator().manual_seed(0)
+    h, w = torch.randn(5, 64, generator=g).bfloat16().to(DEV), torch.randn(300, 64, generator=g).bfloat16().to(DEV)
+    t = torch.tensor([0, 3, 299, -100, 7], device=DEV)
+    with pytest.raises(ValueError, match="softcap"):
+        ops.linear_cross_entropy(h, w, t, softcap=cap * cap)
+    a, b = h.requires_grad_(), w.requires_grad_()
+    got = ops.linear_cross_entropy(a, b, t, softcap=cap)
+    grads = torch.autograd.grad(got.sum(), [a, b])
+    if cap < 1:  # all logits 0, and tanh flat
+        want = torch.where(t == -100, 0.0, math.log(300))
+        assert torch.allclose(got, want, rtol=1e-6) and all((x == 0).all() for x in grads)
+    else:
+        # none: logits of up to 40, whose rounding z = c tanh(u / c) adds some 2^-22 of each
+        want = ops.linear_cross_entropy(a, b, t)
+        assert torch.allclose(got, want, rtol=1e-5, atol=4e-5)
+        for x, y in zip(grads, torch.autograd.grad(want.sum(), [a, b])):
+            assert (x - y).norm() <= 2 * 2 ** -8 * y.norm()
