@@ -45,8 +45,9 @@ int b200_block_norms_bwd(const void* y, int64_t ldy, const void* delta, int64_t 
 int64_t b200_lce_saved_bytes(int T, int Kp);
 // Scratch of the forward pass: a (max, sum) pair per row and column tile.
 int64_t b200_lce_forward_bytes(int T, int V);
-// Scratch of the backward pass: one piece of G (bf16 [T, piece]), then dh's sums.
-int64_t b200_lce_backward_bytes(int T, int K, int piece, int want_dh, int num_sms);
+// Scratch of the backward pass: one piece of G (bf16 [T, piece]), dh's sums, and for dW what
+// the targets' entries lost (fp32 [T, Kp]) with its map (int32 [V]).
+int64_t b200_lce_backward_bytes(int T, int V, int K, int Kp, int piece, int want_dh, int want_dw, int num_sms);
 // Forward. h [T, K] and W [V, K] bf16 (W 16-byte aligned with ldw % 8 == 0), targets
 // int64. Kp: K rounded up to a multiple of 8. loss fp32 [T]; total [1] or null (mean:
 // divided by the scored rows, at least 1).

@@ -64,7 +64,8 @@ struct Args {
   const float* dloss;    // incoming gradient, element token * dloss_stride
   int64_t dloss_stride;
   int mean;              // dloss is of the mean: divide by n
-  const __nv_bfloat16* hc;  // kDw: [T][Kp] scored rows
+  const float* lost;     // kDw: [T][Kp] sums of what the targets' entries of G lost, times h
+  const int* lost_of;    // kDw: [V] their rows, by vocabulary row
   int Kp;
   float2* part;          // kStats: [tiles of 256 columns][T]
   int acc_rows;          // kDh: rows of one part of the fp32 sums (whole half tiles, so that none reaches into the next)
@@ -246,31 +247,22 @@ __device__ __forceinline__ float target_grad(const Args& a, int row) {
   return expm1f(-a.loss[row]) * (1.f - q * q) * row_factor(a, row);
 }
 
-// What the targets' entries of G lost when they were rounded to bf16 goes back to dW
-// where the scored rows are few: over many the roundings average out beside dW's own
-// (2.3e-3 against 1.7e-3 with random weights, 1001 rows), but a few can share one of up
-// to 2^-8. Rows of the batch (bit t) whose target is vocabulary row `col`; a warp's call.
-constexpr int kExactTargets = 64;
-__device__ __forceinline__ uint64_t rows_of_target(const Args& a, int n, int col) {
-  const int lane = threadIdx.x & 31;
-  const int lo = lane < n ? a.target[lane] : -1, hi = lane + 32 < n ? a.target[lane + 32] : -1;
-  uint64_t rows = 0;
-  for (int t = 0; t < 32; ++t) {
-    if (__shfl_sync(0xffffffffu, lo, t) == col) rows |= 1ull << t;
-    if (__shfl_sync(0xffffffffu, hi, t) == col) rows |= 1ull << (t + 32);
-  }
-  return rows;
+// Row of `lost` (lost_targets_kernel) that belongs to vocabulary row `col`, or -1. The map is
+// written for targets only: elsewhere it holds anything, and no row has that target.
+__device__ __forceinline__ int lost_row(const Args& a, int n, int col) {
+  const int r = a.lost_of[col];
+  return (unsigned)r < (unsigned)n && a.target[r] == col ? r : -1;
 }
 // Added to 32 columns (from k0) of dW's row.
-__device__ __forceinline__ void add_lost_targets(const Args& a, uint64_t rows, int k0, uint32_t (&v)[32]) {
-  for (; rows; rows &= rows - 1) {
-    const int t = __ffsll((long long)rows) - 1;
-    const float g = target_grad(a, t), e = g - bf2f(f2bf(g));
-    const __nv_bfloat16* h = a.hc + (int64_t)t * a.Kp + k0;
+__device__ __forceinline__ void add_lost(const Args& a, int r, int k0, uint32_t (&v)[32]) {
+  const float* p = a.lost + (int64_t)r * a.Kp + k0;
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (k0 + j < a.K) v[j] = __float_as_uint(fmaf(e, bf2f(h[j]), __uint_as_float(v[j])));
-  }
+  for (int j = 0; j < 32; j += 4)
+    if (k0 + j < a.Kp) {
+      const float4 x = *reinterpret_cast<const float4*>(p + j);
+      v[j] = __float_as_uint(__uint_as_float(v[j]) + x.x), v[j + 1] = __float_as_uint(__uint_as_float(v[j + 1]) + x.y);
+      v[j + 2] = __float_as_uint(__uint_as_float(v[j + 2]) + x.z), v[j + 3] = __float_as_uint(__uint_as_float(v[j + 3]) + x.w);
+    }
 }
 
 // All pieces (the last may be shorter) and the final sum use the same parts.
@@ -448,8 +440,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
         }
       }
-      uint64_t lost = 0;
-      if (OP == kDw && n <= kExactTargets) lost = rows_of_target(a, n, row < a.nv ? a.v0 + row : -2);
+      int lost = -1;
+      if (OP == kDw && row < a.nv) lost = lost_row(a, n, a.v0 + row);
       // after a wait that ran out (the status word says so) the warp goes on without waiting, so
       // that the barriers among the warps are all met and the kernel ends
       if (!dead) dead = __any_sync(0xffffffffu, !mbar_wait(bar_tfull + 8 * buf, (tile >> 1) & 1, kErrTmemWait));
@@ -554,7 +546,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               uint32_t v[32];
               tmem_ld32(acc + c + hh, v);
               tc_wait_ld();
-              if (lost) add_lost_targets(a, lost, n0 + c + hh, v);
+              if (lost >= 0) add_lost(a, lost, n0 + c + hh, v);
 #pragma unroll
               for (int j = 0; j < 32; j += 2)
                 o[(hh + j) / 2] = pack_bf16x2(__uint_as_float(v[j]) * factor, __uint_as_float(v[j + 1]) * factor);
@@ -762,6 +754,74 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(MergeArgs a) {
   if (threadIdx.x == 0) *a.total = a.mean ? acc / (float)max(n, 1) : acc;
 }
 
+// What the targets' entries of G lose when they are rounded to bf16, as dW misses it: for each
+// target the sum of e_t h_t over its rows in order, e_t = g_t - bf16(g_t). A target's row of dW
+// consists mostly of those entries, however many rows the batch has, so without it their rounding
+// shows beside dW's own (error against 64 bits, 1001 rows with weights, 50257 x 2560: 2.24e-3
+// without, 1.7e-3 with, the output's own rounding; 20 us of 950).
+// CTA (r, y): scored row r, which does the work of its target if it is the first row that has it,
+// and 2048 columns. Finding the rows reads at most n targets for each different one.
+struct LostArgs {
+  Args g;
+  const __nv_bfloat16* hc;  // [T][Kp] scored rows
+  float* lost;              // [T][Kp]: row r for the target that row r is the first of
+  int* lost_of;             // [V]
+};
+constexpr int kLostThreads = 256;
+__global__ void __launch_bounds__(kLostThreads) lost_targets_kernel(const LostArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  __shared__ int found[kLostThreads];
+  __shared__ int warp_n[kLostThreads / 32];
+  const int r = blockIdx.x, n = *a.g.count, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (r >= n) return;
+  const int y = a.g.target[r];
+  if (y < 0) return;
+  // later rows of a frequent target find an earlier one soon
+  for (int t0 = 0; t0 < r; t0 += 4 * kLostThreads) {
+    bool seen = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = t0 + i * kLostThreads + (int)threadIdx.x;
+      seen |= t < r && a.g.target[t] == y;
+    }
+    if (__syncthreads_or(seen)) return;
+  }
+  const int c = (blockIdx.y * kLostThreads + threadIdx.x) * 8;
+  float s[8] = {};
+  for (int t0 = r; t0 < n; t0 += kLostThreads) {
+    const int t = t0 + threadIdx.x;
+    const bool mine = t < n && a.g.target[t] == y;
+    const unsigned b = __ballot_sync(0xffffffffu, mine);
+    if (!__syncthreads_or(mine)) continue;  // also: the list of the rows before has been read
+    if (lane == 0) warp_n[warp] = __popc(b);
+    __syncthreads();
+    int at = __popc(b & ((1u << lane) - 1)), total = 0;
+#pragma unroll
+    for (int i = 0; i < kLostThreads / 32; ++i) {
+      at += i < warp ? warp_n[i] : 0;
+      total += warp_n[i];
+    }
+    if (mine) found[at] = t;
+    __syncthreads();
+    if (c < a.g.Kp)
+      for (int i = 0; i < total; ++i) {
+        const int row = found[i];
+        const float g = target_grad(a.g, row), e = g - bf2f(f2bf(g));
+        const uint4 hv = *reinterpret_cast<const uint4*>(a.hc + (int64_t)row * a.g.Kp + c);
+        const __nv_bfloat16* he = reinterpret_cast<const __nv_bfloat16*>(&hv);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] = fmaf(e, bf2f(he[j]), s[j]);
+      }
+  }
+  if (c < a.g.Kp) {
+    float4* o = reinterpret_cast<float4*>(a.lost + (int64_t)r * a.g.Kp + c);
+    o[0] = make_float4(s[0], s[1], s[2], s[3]);
+    o[1] = make_float4(s[4], s[5], s[6], s[7]);
+  }
+  if (blockIdx.y == 0 && threadIdx.x == 0) a.lost_of[y] = r;
+}
+
 // dh[t] = (sum over the contraction's parts of acc[.][place[t]] + e W[y]) * factor, 0
 // for ignored rows. e is what the target's entry of G lost when it was rounded to bf16:
 // that entry alone is of the size of the whole row, the others are far below it, so
@@ -862,9 +922,11 @@ static int most_parts(int T, int K, int num_sms) {
 static int acc_rows(int T) { return (int)(tiles_of(T, kRowsM) * kRowsM); }
 static int acc_cols(int K) { return (K + 3) / 4 * 4; }
 
-// Scratch of the backward pass: one piece of G (bf16 [T, piece]), then dh's sums.
-int64_t b200_lce_backward_bytes(int T, int K, int piece, int want_dh, int num_sms) {
-  return (int64_t)T * piece * 2 + (want_dh ? (int64_t)most_parts(T, K, num_sms) * acc_rows(T) * acc_cols(K) * 4 : 0);
+// Scratch of the backward pass: one piece of G (bf16 [T, piece]), dh's sums, and for dW what
+// the targets' entries lost (fp32 [T, Kp]) with its map (int32 [V]).
+static int64_t dh_bytes(int T, int K, int num_sms) { return (int64_t)most_parts(T, K, num_sms) * acc_rows(T) * acc_cols(K) * 4; }
+int64_t b200_lce_backward_bytes(int T, int V, int K, int Kp, int piece, int want_dh, int want_dw, int num_sms) {
+  return (int64_t)T * piece * 2 + (want_dh ? dh_bytes(T, K, num_sms) : 0) + (want_dw ? (int64_t)T * Kp * 4 + (int64_t)V * 4 : 0);
 }
 
 struct Saved {
@@ -984,7 +1046,6 @@ int b200_lce_backward(void* saved, const void* W, int64_t ldw, const float* dlos
   a.cap = cap;
   a.inv_cap = cap > 0.f ? 1.f / cap : 0.f;
   a.unbias = unbias_of(K);
-  a.hc = reinterpret_cast<const __nv_bfloat16*>(f.hc);
   a.Kp = Kp;
   void* G = scratch;
   float* acc = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(scratch) + (int64_t)T * piece * 2);
@@ -1000,6 +1061,18 @@ int b200_lce_backward(void* saved, const void* W, int64_t ldw, const float* dlos
   if (dW && (!make_tmap_2d(&g_cols, G, T, piece, piece, 64, 64, 2) || !make_tmap_2d(&h_cols, f.hc, T, Kp, Kp, 64, 64, 2) ||
              !make_tmap_2d(&o_dw, dW, V, K, lddw, kRowsM, 64, 2)))
     return -1;
+  if (dW) {
+    LostArgs l = {};
+    l.lost = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(acc) + (dh ? dh_bytes(T, K, num_sms) : 0));
+    l.lost_of = reinterpret_cast<int*>(l.lost + (int64_t)T * Kp);
+    a.lost = l.lost;
+    a.lost_of = l.lost_of;
+    l.g = a;
+    l.hc = reinterpret_cast<const __nv_bfloat16*>(f.hc);
+    const dim3 grid((unsigned)T, (unsigned)tiles_of(Kp, 8 * kLostThreads));
+    const cudaError_t e = launch_k(lost_targets_kernel, grid, dim3(kLostThreads), 0, st, 1, l);
+    if (e != cudaSuccess) return (int)e;
+  }
   for (int64_t v0 = 0; v0 < V; v0 += piece) {
     a.v0 = (int)v0;
     a.nv = (int)(V - v0 < piece ? V - v0 : piece);

@@ -467,7 +467,8 @@ struct LinearCe : torch::autograd::Function<LinearCe> {
     const Tensor w = aligned_head(w_), g = grads[0].reshape(-1);
     const int sms = num_sms(w.device());
     const Launch on(w);
-    const Tensor scratch = empty(w, {lib.b200_lce_backward_bytes((int)T, (int)K, (int)piece, (int)call[4], sms)}, at::kByte);
+    const int64_t room = lib.b200_lce_backward_bytes((int)T, (int)V, (int)K, (int)Kp, (int)piece, (int)call[4], (int)call[5], sms);
+    const Tensor scratch = empty(w, {room}, at::kByte);
     Tensor dh, dw;
     if (call[4]) dh = empty(w, {T, K}, at::kBFloat16);
     if (call[5]) {  // rows as TMA stores them
