@@ -8,7 +8,7 @@
 //
 // The target's logit stands apart from the sum over the others, so a loss near
 // zero (and p_y - 1 = expm1(-loss)) keeps its digits. It is a dot product in
-// fp32 of its own; the others come from the tensor cores.
+// fp32 of its own; the others come from the tensor cores, in chunks (kChunk).
 //
 // Forward: one product whose tiles leave a (max, sum of exp) pair per row and
 // 256 columns. Backward: the vocabulary in pieces; each forms its logits again
@@ -74,15 +74,7 @@ struct Args {
   int piece, pairs;      // kDh: columns of a whole piece and CTA pairs (choose_parts)
   int most_parts, first;  // kDh: parts the sums have room for; first piece stores, others add
   float cap, inv_cap;    // cap 0: none
-  float unbias;          // factor of the products' results (unbias_of)
 };
-
-// The tensor cores add each 16-deep step into the fp32 accumulator by truncation:
-// products of K terms come out too small by K / 16 steps of about 2^-26 (measured
-// against 64 bits on unit normal operands: 1.9e-7 at K = 256, 8.6e-7 at 1024, 3.8e-6
-// at 4096). Of a mean loss that would be the whole error, so the logits are scaled
-// back by it; what is left has either sign.
-static float unbias_of(int K) { return 1.f + (float)((K + 15) / 16) * (1.f / 67108864.f); }
 
 constexpr int kTileM = 256, kTileN = 256, kStages = 6;  // of a pair of CTAs
 constexpr int kRowsM = kTileM / 2, kRowsN = kTileN / 2;   // a CTA's share of either operand
@@ -96,6 +88,22 @@ constexpr int kEpiWarps = 8;  // (four: the capped G of 901 x 50257 x 2560 took 
 constexpr int kHalfN = kTileN / 2;
 constexpr int kGroupM = 16;  // row tiles walked per column tile before the next: W is read once per 16 x 256 rows, h stays in L2
 static_assert(kSmem <= 227 * 1024, "shared memory plan exceeds the per-CTA limit");
+
+// The tensor cores add each 16-deep step into the fp32 accumulator by truncation, so a sum
+// comes out too small by up to half a step of what it had reached, each time: without more the
+// loss of logits up to 20 at K = 4096 is off by 6.7e-6 on normal operands and 2.9e-4 where all
+// products are positive (fp32 sums rounded to nearest: 9e-7 and 2e-5), and not at all where the
+// sums are exact. So the logits are summed a chunk of blocks of 64 at a time, and the chunks
+// added up, rounded to nearest, in the registers of the epilogue's threads, half a row of a
+// tile each. Reading the accumulators more often costs the products their time: statistics of
+// 512 rows of 151936 x 4096 457 us in one chunk, 472 in chunks 1024 deep, 490 in 512 (which
+// brings the errors to those of rounded sums), 540 in 256. G is rounded to bf16: 1024 there
+// (a full step of 4096 rows 14.9 ms in one chunk, 15.5 as it is, 15.8 with 512 for both).
+template <int OP>
+constexpr int kChunk = OP == 0 ? 8 : OP == 1 ? 16 : 1 << 30;  // kStats, kGrad; the others' results are rounded to bf16
+// Those threads need more registers than 168, the share of 384: the other four warps give some of theirs.
+constexpr int kRegsMax = 168, kRegsRest = 56, kRegsEpi = 224;
+static_assert(128 * kRegsRest + 256 * kRegsEpi <= kThreads * kRegsMax, "more registers than the block is launched with");
 
 // --- tcgen05 on a pair of CTAs ---
 __device__ __forceinline__ void tmem_alloc2(uint32_t dst_smem, uint32_t ncols) {
@@ -271,11 +279,17 @@ __device__ __forceinline__ int dh_parts(const Args& a, int n) {
   return choose_parts(tiles, min(a.piece, a.V) / 64, a.pairs, a.most_parts);
 }
 
+template <int REGS>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS)); }
+template <int REGS>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS)); }
+
 template <int OP>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                 const __grid_constant__ CUtensorMap tmO, const Args a) {
   constexpr bool A_MN = OP == kDw, B_MN = OP == kDh || OP == kDw;
+  constexpr bool kLogits = OP == kStats || OP == kGrad;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
@@ -333,104 +347,148 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   w.total = w.mt * w.nt * w.splits;
   const int kb_per = (kb_total + w.splits - 1) / w.splits;
 
-  if (warp == 0) {
-    if (lane == 0) {
-      // both operands are read by several pairs and rounds (4096 rows: 15.9 ms a step; 16.2 with W
-      // evict-normal, 16.3 evict-first)
-      const uint64_t pol = l2_policy_evict_last();
-      int it = 0;
-      bool ok = true;
-      for (int t = pair; ok && t < w.total; t += pairs) {
-        int m, nn, s;
-        w.at(t, m, nn, s);
-        const int m0 = m * kTileM + rank * kRowsM, n0 = nn * kTileN + rank * kRowsN;
-        const int kb0 = s * kb_per, kb1 = min(kb_total, kb0 + kb_per);
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int st = it % kStages, r = it / kStages;
-          if (r > 0 && !mbar_wait(bar_empty + 8 * st, (r - 1) & 1, kErrGemmWait)) {
-            ok = false;
-            break;
-          }
-          const uint32_t sa = sbase + st * kStageBytes, sb = sa + kABytes;
-          const uint32_t bar = in_leader(bar_full + 8 * st);
-          if (rank == 0) mbar_arrive_expect_tx(bar_full + 8 * st, 2 * kStageBytes);
-          const int kc = kb * 64;
-          if constexpr (A_MN) {
+  if (warp < 4) {
+    if constexpr (kLogits) regs_down<kRegsRest>();
+    if (warp == 0) {
+      if (lane == 0) {
+        // both operands are read by several pairs and rounds (4096 rows: 15.9 ms a step; 16.2 with W
+        // evict-normal, 16.3 evict-first)
+        const uint64_t pol = l2_policy_evict_last();
+        int it = 0;
+        bool ok = true;
+        for (int t = pair; ok && t < w.total; t += pairs) {
+          int m, nn, s;
+          w.at(t, m, nn, s);
+          const int m0 = m * kTileM + rank * kRowsM, n0 = nn * kTileN + rank * kRowsN;
+          const int kb0 = s * kb_per, kb1 = min(kb_total, kb0 + kb_per);
+          for (int kb = kb0; kb < kb1; ++kb, ++it) {
+            const int st = it % kStages, r = it / kStages;
+            if (r > 0 && !mbar_wait(bar_empty + 8 * st, (r - 1) & 1, kErrGemmWait)) {
+              ok = false;
+              break;
+            }
+            const uint32_t sa = sbase + st * kStageBytes, sb = sa + kABytes;
+            const uint32_t bar = in_leader(bar_full + 8 * st);
+            if (rank == 0) mbar_arrive_expect_tx(bar_full + 8 * st, 2 * kStageBytes);
+            const int kc = kb * 64;
+            if constexpr (A_MN) {
 #pragma unroll
-            for (int j = 0; j < kRowsM / 64; ++j) tma_load_pair(sa + j * 8192, &tmA, bar, m0 + 64 * j, kc, pol);
-          } else {
-            tma_load_pair(sa, &tmA, bar, kc, m0, pol);
-          }
-          if constexpr (B_MN) {
-            const int row = OP == kDh ? a.v0 + kc : kc;
+              for (int j = 0; j < kRowsM / 64; ++j) tma_load_pair(sa + j * 8192, &tmA, bar, m0 + 64 * j, kc, pol);
+            } else {
+              tma_load_pair(sa, &tmA, bar, kc, m0, pol);
+            }
+            if constexpr (B_MN) {
+              const int row = OP == kDh ? a.v0 + kc : kc;
 #pragma unroll
-            for (int j = 0; j < kRowsN / 64; ++j) tma_load_pair(sb + j * 8192, &tmB, bar, n0 + 64 * j, row, pol);
-          } else {
-            tma_load_pair(sb, &tmB, bar, kc, a.v0 + n0, pol);
+              for (int j = 0; j < kRowsN / 64; ++j) tma_load_pair(sb + j * 8192, &tmB, bar, n0 + 64 * j, row, pol);
+            } else {
+              tma_load_pair(sb, &tmB, bar, kc, a.v0 + n0, pol);
+            }
           }
         }
+        // every stage filled here has been consumed before the CTA leaves, so that no copy
+        // and no arrival on its barriers is still under way
+        for (int i = max(0, it - kStages); i < it; ++i)
+          mbar_wait(bar_empty + 8 * (i % kStages), (i / kStages) & 1, kErrGemmWait);
       }
-      // every stage filled here has been consumed before the CTA leaves, so that no copy
-      // and no arrival on its barriers is still under way
-      for (int i = max(0, it - kStages); i < it; ++i)
-        mbar_wait(bar_empty + 8 * (i % kStages), (i / kStages) & 1, kErrGemmWait);
-    }
-  } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
-      constexpr uint32_t idesc = umma_idesc_bf16(kTileM, kTileN, A_MN, B_MN);
-      int it = 0, tile = 0;
-      bool ok = true;
-      for (int t = pair; ok && t < w.total; t += pairs, ++tile) {
-        int m, nn, s;
-        w.at(t, m, nn, s);
-        const int kb0 = s * kb_per, kb1 = min(kb_total, kb0 + kb_per);
-        const int buf = tile & 1;
-        if (!mbar_wait(bar_tempty + 8 * buf, ((tile >> 1) & 1) ^ 1, kErrTmemWait)) break;
-        tc_fence_after();
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int st = it % kStages, r = it / kStages;
-          if (!mbar_wait(bar_full + 8 * st, r & 1, kErrGemmWait)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t sa = sbase + st * kStageBytes, sb = sa + kABytes;
-          // 16 deep per instruction: K-major tiles step 32 bytes along their rows, MN-major ones 16
-          // rows of 128 bytes
-          const uint64_t ad = A_MN ? umma_desc_mn_sw128(sa, 8192, 1024) : umma_desc_k_sw128(sa, 1024);
-          const uint64_t bd = B_MN ? umma_desc_mn_sw128(sb, 8192, 1024) : umma_desc_k_sw128(sb, 1024);
+    } else if (warp == 1) {
+      if (lane == 0 && rank == 0) {
+        constexpr uint32_t idesc = umma_idesc_bf16(kTileM, kTileN, A_MN, B_MN);
+        int it = 0, fill = 0;  // fill: chunks into an accumulator
+        bool ok = true;
+        for (int t = pair; ok && t < w.total; t += pairs) {
+          int m, nn, s;
+          w.at(t, m, nn, s);
+          const int kb0 = s * kb_per, kb1 = min(kb_total, kb0 + kb_per);
+          int kb = kb0;
+          do {  // once where nothing is contracted
+            const int first = kb, last = kb1 - kb > kChunk<OP> ? kb + kChunk<OP> : kb1, buf = fill & 1;
+            if (!mbar_wait(bar_tempty + 8 * buf, ((fill >> 1) & 1) ^ 1, kErrTmemWait)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            for (; kb < last; ++kb, ++it) {
+              const int st = it % kStages, r = it / kStages;
+              if (!mbar_wait(bar_full + 8 * st, r & 1, kErrGemmWait)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              const uint32_t sa = sbase + st * kStageBytes, sb = sa + kABytes;
+              // 16 deep per instruction: K-major tiles step 32 bytes along their rows, MN-major ones 16
+              // rows of 128 bytes
+              const uint64_t ad = A_MN ? umma_desc_mn_sw128(sa, 8192, 1024) : umma_desc_k_sw128(sa, 1024);
+              const uint64_t bd = B_MN ? umma_desc_mn_sw128(sb, 8192, 1024) : umma_desc_k_sw128(sb, 1024);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mma2_f16(tmem + buf * kTileN, ad + (A_MN ? 128 : 2) * k, bd + (B_MN ? 128 : 2) * k, idesc,
-                     (kb > kb0 || k > 0) ? 1u : 0u);
-          commit2(bar_empty + 8 * st);
+              for (int k = 0; k < 4; ++k)
+                mma2_f16(tmem + buf * kTileN, ad + (A_MN ? 128 : 2) * k, bd + (B_MN ? 128 : 2) * k, idesc,
+                         (kb > first || k > 0) ? 1u : 0u);
+              commit2(bar_empty + 8 * st);
+            }
+            commit2(bar_tfull + 8 * buf);
+            ++fill;
+          } while (ok && kb < kb1);
         }
-        commit2(bar_tfull + 8 * buf);
       }
     }
-  } else if (warp >= 4) {
+  } else {
+    if constexpr (kLogits) regs_up<kRegsEpi>();
     const int r = (warp & 3) * 32 + lane;  // row of the CTA's half tile = tensor-memory lane
     const int half = (warp - 4) >> 2, left = half * kHalfN;
     const bool first_thread = (threadIdx.x & 127) == 0;  // of the half
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    // logits as exponents of two, before the cap if there is one
-    const float to_log2 = a.cap > 0.f ? kLog2e : kLog2e * a.unbias, to_cap = a.inv_cap * a.unbias;
     const float factor = OP == kDw ? common_factor(a, n) : 1.f;
     const uint32_t release = in_leader(bar_tempty);
-    int tile = 0;
+    int tile = 0, fill = 0;
     bool dead = false;
+    // The next full accumulator (its left column of this half). After a wait that ran out (the
+    // status word says so) the warp goes on without waiting, so that the barriers among the
+    // warps are all met and the kernel ends.
+    auto filled = [&]() -> uint32_t {
+      const int buf = fill & 1;
+      if (!dead) dead = __any_sync(0xffffffffu, !mbar_wait(bar_tfull + 8 * buf, (fill >> 1) & 1, kErrTmemWait));
+      tc_fence_after();
+      return tmem + lanes + buf * kTileN + left;
+    };
+    auto emptied = [&] {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_cluster(release + 8 * (fill & 1));
+      ++fill;
+    };
+    // 128 bytes of a row (64 bf16 or 32 fp32) through the half's staging buffer in the 128-byte
+    // swizzle, stored by one thread while the next ones are formed. c: first column in the
+    // tile; row0: first row; a box that starts outside is not stored, what reaches past the
+    // end of another is not written.
+    auto put = [&](const uint32_t (&o)[32], int col, int row0, bool any_row) {
+      const uint32_t stage = out_smem + half * kOutBytes;
+      if (first_thread) bulk_wait_read<0>();  // the last store has left the buffer
+      half_barrier(half);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + sw128_offset(r, 16 * j)), "r"(o[4 * j]),
+                     "r"(o[4 * j + 1]), "r"(o[4 * j + 2]), "r"(o[4 * j + 3])
+                     : "memory");
+      fence_proxy_async_smem();
+      half_barrier(half);
+      if (first_thread) {
+        if (any_row) {
+          if (OP != kDh || a.first) tma_store(&tmO, stage, col, row0);
+          else tma_add_f32(&tmO, stage, col, row0);
+        }
+        bulk_commit();
+      }
+    };
     for (int t = pair; t < w.total; t += pairs, ++tile) {
       int m, nn, s;
       w.at(t, m, nn, s);
       const int m0 = m * kTileM + rank * kRowsM, row = m0 + r, n0 = nn * kTileN;
-      const int buf = tile & 1;
-      const uint32_t acc = tmem + lanes + buf * kTileN;
-      const bool empty = s * kb_per >= kb_total;  // nothing contracted: the product is zero
-      const int cols = min(kTileN, (OP == kStats || OP == kGrad ? a.nv : a.K) - n0);
+      const int cols = min(kTileN, (kLogits ? a.nv : a.K) - n0);
       const int end = min(left + kHalfN, cols);  // this half: columns left .. end - 1 of the tile, or none
-      int target = -1;
-      float shift = 0.f, dl = 0.f, at_target = 0.f;
-      if constexpr (OP == kStats || OP == kGrad) {
+      if constexpr (kLogits) {
+        int target = -1;
+        float shift = 0.f, dl = 0.f, at_target = 0.f;
         if (row < n) {
           target = a.target[row] - (a.v0 + n0);  // its column in this tile, if within 0 .. 255
           if constexpr (OP == kGrad) {
@@ -439,105 +497,119 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             at_target = target_grad(a, row);
           }
         }
-      }
-      int lost = -1;
-      if (OP == kDw && row < a.nv) lost = lost_row(a, n, a.v0 + row);
-      // after a wait that ran out (the status word says so) the warp goes on without waiting, so
-      // that the barriers among the warps are all met and the kernel ends
-      if (!dead) dead = __any_sync(0xffffffffu, !mbar_wait(bar_tfull + 8 * buf, (tile >> 1) & 1, kErrTmemWait));
-      tc_fence_after();
-      if constexpr (OP == kStats) {
-        float mx = -INFINITY, sum = 0.f;
-#pragma unroll 1
-        for (int c = left; c < end; c += 32) {
-          uint32_t v[32];
-          tmem_ld32(acc + c, v);
+        // this half row of the tile: the chunks' sums
+        uint32_t z[kHalfN];
+        {
+          const uint32_t acc = filled();
+#pragma unroll
+          for (int i = 0; i < kHalfN; i += 32) tmem_ld32(acc + i, z + i);
           tc_wait_ld();
-          if (a.cap > 0.f) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(a.cap * tanhf(__uint_as_float(v[j]) * to_cap));
-          }
-          // columns past the vocabulary and the target's take no part
-          if (c + 32 > cols || (unsigned)(target - c) < 32u) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (c + j >= cols || c + j == target) v[j] = 0xff800000u;
-          }
-          float cm = __uint_as_float(v[0]);
-#pragma unroll
-          for (int j = 1; j < 32; ++j) cm = fmaxf(cm, __uint_as_float(v[j]));
-          const float m2 = fmaxf(mx, cm);
-          if (m2 > -INFINITY) {
-            const float off = m2 * to_log2;
-            sum = mx > -INFINITY ? sum * ex2(mx * to_log2 - off) : sum;  // 0, or NaN that stays
-            float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              s0 += ex2(fmaf(__uint_as_float(v[j]), to_log2, -off));
-              s1 += ex2(fmaf(__uint_as_float(v[j + 1]), to_log2, -off));
-            }
-            sum += s0 + s1;
-            mx = m2;
-          } else {
-            // only -inf or NaN so far: NaN has to reach the sum
-#pragma unroll
-            for (int j = 0; j < 32; ++j) sum += __uint_as_float(v[j]) == -INFINITY ? 0.f : __uint_as_float(v[j]);
-          }
+          emptied();
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) arrive_cluster(release + 8 * buf);
-        if (!(a.cap > 0.f)) mx *= a.unbias;
-        // the right half's pair joins the left's; the buffers alternate between tiles, and the barrier
-        // of the next tile is passed before one is written again
-        float2* pairs_smem = reinterpret_cast<float2*>(smem + kStages * kStageBytes) + (tile & 1) * kRowsM;
-        if (half) pairs_smem[r] = make_float2(mx, sum);
-        epi_barrier();
-        if (!half && row < n) {
-          const float2 p = pairs_smem[r];
-          join(mx, sum, p.x, p.y);
-          a.part[(int64_t)nn * a.T + row] = make_float2(mx, sum);
+        for (int kb = kChunk<OP>; kb < kb_total; kb += kChunk<OP>) {
+          const uint32_t acc = filled();
+#pragma unroll
+          for (int i = 0; i < kHalfN; i += 32) {
+            uint32_t v[32];
+            tmem_ld32(acc + i, v);
+            tc_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) z[i + j] = __float_as_uint(__uint_as_float(z[i + j]) + __uint_as_float(v[j]));
+          }
+          emptied();
+        }
+        if constexpr (OP == kStats) {
+          float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < kHalfN; i += 32) {
+            const int c = left + i;
+            uint32_t* v = z + i;
+            if (c >= end) continue;
+            if (a.cap > 0.f) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(a.cap * tanhf(__uint_as_float(v[j]) * a.inv_cap));
+            }
+            // columns past the vocabulary and the target's take no part
+            if (c + 32 > cols || (unsigned)(target - c) < 32u) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (c + j >= cols || c + j == target) v[j] = 0xff800000u;
+            }
+            float cm = __uint_as_float(v[0]);
+#pragma unroll
+            for (int j = 1; j < 32; ++j) cm = fmaxf(cm, __uint_as_float(v[j]));
+            const float m2 = fmaxf(mx, cm);
+            if (m2 > -INFINITY) {
+              const float off = m2 * kLog2e;
+              sum = mx > -INFINITY ? sum * ex2(mx * kLog2e - off) : sum;  // 0, or NaN that stays
+              float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+              for (int j = 0; j < 32; j += 2) {
+                s0 += ex2(fmaf(__uint_as_float(v[j]), kLog2e, -off));
+                s1 += ex2(fmaf(__uint_as_float(v[j + 1]), kLog2e, -off));
+              }
+              sum += s0 + s1;
+              mx = m2;
+            } else {
+              // only -inf or NaN so far: NaN has to reach the sum
+#pragma unroll
+              for (int j = 0; j < 32; ++j) sum += __uint_as_float(v[j]) == -INFINITY ? 0.f : __uint_as_float(v[j]);
+            }
+          }
+          // the right half's pair joins the left's; the buffers alternate between tiles, and the barrier
+          // of the next tile is passed before one is written again
+          float2* pairs_smem = reinterpret_cast<float2*>(smem + kStages * kStageBytes) + (tile & 1) * kRowsM;
+          if (half) pairs_smem[r] = make_float2(mx, sum);
+          epi_barrier();
+          if (!half && row < n) {
+            const float2 p = pairs_smem[r];
+            join(mx, sum, p.x, p.y);
+            a.part[(int64_t)nn * a.T + row] = make_float2(mx, sum);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kHalfN; i += 64) {
+            const int c = left + i;
+            uint32_t* v = z + i;
+            if (c >= end) continue;
+            if (a.cap > kFastTanhCap) {
+#pragma unroll
+              for (int j = 0; j < 64; ++j) v[j] = __float_as_uint(tanhf(__uint_as_float(v[j]) * a.inv_cap));
+            } else if (a.cap > 0.f) {
+#pragma unroll
+              for (int j = 0; j < 64; ++j) v[j] = __float_as_uint(tanh_fast(__uint_as_float(v[j]) * a.inv_cap));
+            }
+            const int rel = target - c;
+            uint32_t o[32];
+#pragma unroll
+            for (int j = 0; j < 64; j += 2) {
+              float p[2];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                float u = __uint_as_float(v[j + e]), slope = dl;
+                if (a.cap > 0.f) {  // u is the tanh
+                  slope *= 1.f - u * u;
+                  u *= a.cap;
+                }
+                p[e] = ex2(fmaf(u, kLog2e, -shift)) * slope;
+                if (rel == j + e) p[e] = at_target;
+                if (row >= n || c + j + e >= cols) p[e] = 0.f;
+              }
+              o[j / 2] = pack_bf16x2(p[0], p[1]);
+            }
+            put(o, n0 + c, m0, m0 < n);
+          }
         }
       } else {
-        // 128 bytes of a row at a time (64 bf16 or 32 fp32) through the half's staging buffer in the
-        // 128-byte swizzle, stored by one thread while the next ones are formed
+        const bool empty = s * kb_per >= kb_total;  // nothing contracted: the product is zero
+        int lost = -1;
+        if (OP == kDw && row < a.nv) lost = lost_row(a, n, a.v0 + row);
+        const uint32_t acc = filled() - left;
         constexpr int kStep = OP == kDh ? 32 : 64;
-        const bool any_row = OP == kDw ? m0 < a.nv : m0 < n;
 #pragma unroll 1
         for (int c = left; c < end; c += kStep) {
           uint32_t o[32];
-          if constexpr (OP == kGrad) {
-#pragma unroll
-            for (int hh = 0; hh < 64; hh += 32) {
-              uint32_t v[32];
-              tmem_ld32(acc + c + hh, v);
-              tc_wait_ld();
-              const int rel = target - (c + hh);
-              if (a.cap > kFastTanhCap) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(tanhf(__uint_as_float(v[j]) * to_cap));
-              } else if (a.cap > 0.f) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(tanh_fast(__uint_as_float(v[j]) * to_cap));
-              }
-#pragma unroll
-              for (int j = 0; j < 32; j += 2) {
-                float p[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  float z = __uint_as_float(v[j + e]), slope = dl;
-                  if (a.cap > 0.f) {  // z is the tanh
-                    slope *= 1.f - z * z;
-                    z *= a.cap;
-                  }
-                  p[e] = ex2(fmaf(z, to_log2, -shift)) * slope;
-                  if (rel == j + e) p[e] = at_target;
-                  if (row >= n || c + hh + j + e >= cols) p[e] = 0.f;
-                }
-                o[(hh + j) / 2] = pack_bf16x2(p[0], p[1]);
-              }
-            }
-          } else if constexpr (OP == kDh) {
+          if constexpr (OP == kDh) {
             tmem_ld32(acc + c, o);
             tc_wait_ld();
           } else {
@@ -552,33 +624,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 o[(hh + j) / 2] = pack_bf16x2(__uint_as_float(v[j]) * factor, __uint_as_float(v[j + 1]) * factor);
             }
           }
-          if (OP != kGrad && empty) {
+          if (empty) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) o[j] = 0u;
           }
-          const uint32_t stage = out_smem + half * kOutBytes;
-          if (first_thread) bulk_wait_read<0>();  // the last store has left the buffer
-          half_barrier(half);
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + sw128_offset(r, 16 * j)), "r"(o[4 * j]),
-                         "r"(o[4 * j + 1]), "r"(o[4 * j + 2]), "r"(o[4 * j + 3])
-                         : "memory");
-          fence_proxy_async_smem();
-          half_barrier(half);
-          if (first_thread) {
-            if (any_row) {  // a box that starts inside; what reaches past the end is not written
-              if constexpr (OP == kGrad) tma_store(&tmO, stage, n0 + c, m0);
-              else if constexpr (OP == kDw) tma_store(&tmO, stage, n0 + c, a.v0 + m0);
-              else if (a.first) tma_store(&tmO, stage, n0 + c, s * a.acc_rows + m0);
-              else tma_add_f32(&tmO, stage, n0 + c, s * a.acc_rows + m0);
-            }
-            bulk_commit();
-          }
+          if constexpr (OP == kDh) put(o, n0 + c, s * a.acc_rows + m0, m0 < n);
+          else put(o, n0 + c, a.v0 + m0, m0 < a.nv);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) arrive_cluster(release + 8 * buf);
+        emptied();
       }
     }
     if (OP != kStats && first_thread) bulk_wait_all();
@@ -883,12 +936,25 @@ __global__ void __launch_bounds__(256) finish_dh_kernel(const FinishArgs a) {
     *o = f2bf(s[0]);
 }
 
+// setmaxnreg.inc would wait for good for registers that the block was not launched with.
+template <int OP>
+static int split_fits() {
+  static const int rc = [] {
+    cudaFuncAttributes f;
+    const cudaError_t e = cudaFuncGetAttributes(&f, gemm_kernel<OP>);
+    return e != cudaSuccess ? (int)e : f.numRegs < kRegsMax ? (int)cudaErrorInvalidKernelImage : 0;
+  }();
+  return rc;
+}
+
 template <int OP>
 static int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& to, const Args& a, int64_t tiles,
                        int num_sms, cudaStream_t st) {
   if (tiles <= 0) return 0;
   if (tiles > 0x7FFFFFFFll - 1024) return -1;
   if (int e = smem_attr_once<gemm_kernel<OP>>(kSmem)) return e;
+  if (OP == kStats || OP == kGrad)
+    if (int e = split_fits<OP>()) return e;
   const int grid = (int)(tiles < num_sms / 2 ? tiles : num_sms / 2);
   cudaError_t e = launch_k(gemm_kernel<OP>, dim3(2 * grid), dim3(kThreads), kSmem, st, 1, ta, tb, to, a);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
@@ -994,7 +1060,6 @@ int b200_lce_forward(const void* h, int64_t ldh, const void* W, int64_t ldw, con
   a.nv = V;
   a.cap = p.cap;
   a.inv_cap = p.inv_cap;
-  a.unbias = unbias_of(K);
   CUtensorMap ta, tb;
   if (!make_tmap_2d(&ta, f.hc, T, Kp, Kp, kRowsM, 64, 2) || !make_tmap_2d(&tb, W, V, K, ldw, kRowsN, 64, 2)) return -1;
   if (int r = launch_gemm<kStats>(ta, tb, ta, a, tiles_of(T, kTileM) * tiles_of(V, kTileN), num_sms, st)) return r;
@@ -1045,7 +1110,6 @@ int b200_lce_backward(void* saved, const void* W, int64_t ldw, const float* dlos
   a.most_parts = most_parts(T, K, num_sms);
   a.cap = cap;
   a.inv_cap = cap > 0.f ? 1.f / cap : 0.f;
-  a.unbias = unbias_of(K);
   a.Kp = Kp;
   void* G = scratch;
   float* acc = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(scratch) + (int64_t)T * piece * 2);
