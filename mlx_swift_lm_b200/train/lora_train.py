@@ -122,7 +122,7 @@ def loss_fn(model, lora: TrainableLoRA | None, inputs, targets, lengths, trainin
         h = train_hidden(model, inputs, lora, training)
         if not isinstance(model.lm_head, torch.Tensor):
             raise ValueError("the fused loss needs a dense head")
-        scored = torch.where(mask, targets, -100).to(h.device)
+        scored = torch.where(mask.to(h.device), targets.to(h.device), -100)
         loss = ops.linear_cross_entropy(h.to(model.lm_head.dtype), model.lm_head, scored,
                                         softcap=model.cfg.final_logit_softcap, reduction="mean")
         return loss, int(mask.sum())
