@@ -147,6 +147,8 @@ def ptr(t: torch.Tensor | None):
 
 def stream_ptr(device=None) -> int:
     """Handle of torch's current stream on `device` (None: the current device)."""
+    if isinstance(device, str):
+        device = torch.device(device)
     index = device.index if isinstance(device, torch.device) else device
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
