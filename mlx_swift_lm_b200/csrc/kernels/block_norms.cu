@@ -242,6 +242,10 @@ __global__ void __launch_bounds__(1024, 1) block_norms_kernel(const BlockNormArg
 // no registers; those hold the weights instead. 0 (unaligned rows, and rows too wide
 // for two stages): straight from global memory. 8192 x 4096 bf16 (403 MB): 95 us from
 // global memory, 81 us (5.0 TB/s) staged, bound by the sums' round trips between rows.
+// The other instantiations pay for registers: at 64 a thread the unstaged ones and the staged
+// gated ones of 1024 threads spill 40 - 164 bytes, and rows of more than 1024 groups (above 8192
+// columns of 16 bits, 4096 of fp32), four or eight groups a thread, 0.8 - 1.4 KB: 4096 x 5120
+// fp32 815 us (0.6 TB/s) where 4096 x 4096 takes 79, 4096 x 12288 bf16 946 us.
 template <typename T, bool VEC, int E, int STAGES>
 struct BwdRows {
   const BlockNormArgs& a;

@@ -40,11 +40,12 @@ __device__ __forceinline__ void draw(uint32_t (&c)[4], const DropoutArgs& a, uns
   philox_4x32_10(c, a.seed);
 }
 
-// Aligned rows: a thread owns a unit at a time, 16-byte loads and stores. Bound by the
-// instructions of the draw at 16-bit types (120 for eight elements with their
-// conversions; 8192 x 4096 bf16 27 us, 5.0 TB/s, the SMs issuing 57 % of the time),
-// by memory at fp32. Two units a thread were slower (35 us: half the warps). `cut` is compared in the upper half of a word, so
-// that the high halves need no shift.
+// Aligned rows: a thread owns a unit at a time, 16-byte loads and stores. At 16-bit
+// types a unit takes 120 instructions with its conversions: 8192 x 4096 bf16 27 us, which
+// is 76 % of the measured memory rate with the SMs issuing 57 % of the time, so that neither
+// is used up; a thread's load, draw and store follow one another. fp32: 48 us (5.5 TB/s), bound
+// by memory. Two units a thread were slower (35 us for bf16: half the warps). `cut` is compared
+// in the upper half of a word, so that the high halves need no shift.
 template <typename T, bool RES>
 __global__ void __launch_bounds__(256) dropout_vec_kernel(const DropoutArgs a) {
   pdl_launch_dependents();

@@ -31,10 +31,10 @@
 // shared memory by TMA; the fp32 sums of dh are added up in L2 by its reduction.
 //
 // Bound by the tensor cores and, in a loop, by the power cap that slows their clock.
-// 4096 x 151936 x 4096: statistics 3.3 ms, G 3.6, dh 3.5, dW 3.6 in a cold burst
-// (1.42 - 1.55 PFLOP/s), 15.0 - 16.2 ms in all when repeated (1.26 - 1.36 PFLOP/s
-// over the four products). With one CTA per 128 x 256 tile and stores from registers
-// the step took 21.8 ms (dW's part alone 10).
+// 4096 rows, 32768 x 4096 head, single passes: statistics 745 us, G 757, dh 724, dW 754
+// (1.45 - 1.52 PFLOP/s); 151936 x 4096 head: 14.7 - 15.9 ms in all when repeated (1.28 -
+// 1.39 PFLOP/s over the four products). With one CTA per 128 x 256 tile and stores from
+// registers the step took 21.8 ms (dW's part alone 10).
 #include "b200_common.cuh"
 #include "b200_train.h"
 
@@ -84,7 +84,9 @@ constexpr int kBars = 2 * kStages + 4;
 constexpr int kBarOffset = kStages * kStageBytes + 2 * kOutBytes;
 constexpr int kSmem = kBarOffset + kBars * 8 + 16 + 1024;  // kStats keeps its pairs in the staging buffers
 constexpr int kThreads = 384;
-constexpr int kEpiWarps = 8;  // (four: the capped G of 901 x 50257 x 2560 took 312 us, not 254) two for each quarter of the lanes: one takes the left half of the columns, one the right
+// Epilogue: two warps for each quarter of the lanes, one for the left half of the columns, one for
+// the right (with four warps the capped G of 901 x 50257 x 2560 took 312 us for 254).
+constexpr int kEpiWarps = 8;
 constexpr int kHalfN = kTileN / 2;
 constexpr int kGroupM = 16;  // row tiles walked per column tile before the next: W is read once per 16 x 256 rows, h stays in L2
 static_assert(kSmem <= 227 * 1024, "shared memory plan exceeds the per-CTA limit");

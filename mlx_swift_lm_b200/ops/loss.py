@@ -12,9 +12,9 @@ from . import _autograd, _lib
 from . import reference as ref
 
 # Bytes of one piece of the logits' gradient. Larger pieces mean fewer passes over the
-# fp32 sums of dh, smaller ones stay nearer the L2 (4096 rows of a 151936 x 4096 head,
-# both gradients: 64 MB 16.1 ms, 128 MB 15.3, 256 MB 15.5, 1 GB 15.9; frozen head, 2048
-# rows: 5.4, 5.1, 5.0, 5.0). A piece is never narrower than MIN_PIECE columns.
+# fp32 sums of dh (4096 rows of a 151936 x 4096 head, both gradients: 64 MB 15.5 ms,
+# 128 MB 15.2, 256 MB 15.0, 1 GB 14.7; frozen head, 2048 rows: 4.85, 4.70, 4.65, 4.60):
+# four times the memory for 2 % is not taken. A piece is never narrower than MIN_PIECE columns.
 PIECE_BYTES = 256 << 20
 MIN_PIECE = 8192
 
