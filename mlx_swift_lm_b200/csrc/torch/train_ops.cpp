@@ -95,9 +95,12 @@ void same_device(const char* what, const Tensor& a, const Tensor& b) {
   if (b.defined()) TORCH_CHECK_VALUE(a.device() == b.device(), what, ": tensors on ", a.device(), " and ", b.device());
 }
 
+// t as it stands in memory: a lazily negated view (complex numbers' .conj().imag) becomes a tensor.
+Tensor plain(const Tensor& t) { return t.defined() ? t.resolve_neg() : t; }
 // t [..., width] as [rows, width] with neighbouring columns: a view where the
 // strides allow it, else a copy. width > 0.
-Tensor rows2d(const Tensor& t, int64_t width) {
+Tensor rows2d(const Tensor& t_, int64_t width) {
+  const Tensor t = plain(t_);
   Tensor r = t.dim() == 2 ? t : t.reshape({-1, width});
   return width <= 1 || r.stride(1) == 1 ? r : r.contiguous();
 }
@@ -213,7 +216,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
 
 Maybe dropout(const Tensor& x, double p, uint64_t seed, uint64_t offset, const Maybe& offset_t,
                               const Maybe& residual_) {
-  const Tensor residual = opt(residual_), off = opt(offset_t);
+  const Tensor residual = opt(residual_), off = plain(opt(offset_t));
   TORCH_CHECK_VALUE(p >= 0.0 && p <= 1.0, "dropout probability ", p, " is not in [0, 1]");
   elem_code(x, "dropout");
   if (residual.defined()) {
@@ -246,9 +249,9 @@ struct NormCall {
 };
 
 Tensor gate_rows(const Tensor& gate, int64_t kind, int64_t H) {
-  return !gate.defined() ? gate : kind == kElement ? rows2d(gate, H) : gate.contiguous();
+  return !gate.defined() ? gate : kind == kElement ? rows2d(gate, H) : plain(gate).contiguous();
 }
-Tensor packed(const Tensor& w) { return w.defined() ? w.contiguous() : w; }
+Tensor packed(const Tensor& w) { return w.defined() ? plain(w).contiguous() : w; }
 
 // An in-place call reads `t` ([rows, cols] with rows `ld` apart) while other CTAs write rows of
 // x. That is sound where t's elements are none of x's, or (aligned: one for each of x's) where
@@ -386,6 +389,7 @@ std::optional<std::pair<Tensor, Maybe>> block_norms(
                     (x.requires_grad() || delta.requires_grad() || wants_grad(post) || wants_grad(pre) || wants_grad(gate));
   if (inplace) {
     TORCH_CHECK_VALUE(!grad, "block_norms: inplace takes no gradients");
+    TORCH_CHECK_VALUE(!x.is_neg(), "block_norms: inplace on a lazily negated view");
     const Tensor rows = x.view({-1, H});
     TORCH_CHECK_VALUE(x.numel() == 0 || ((H == 1 || rows.stride(1) == 1) && (rows.size(0) == 1 || rows.stride(0) >= H)),
                       "block_norms: inplace needs rows of neighbouring columns that do not overlap");
@@ -422,7 +426,7 @@ enum Reduction { kEach = 0, kSum = 1, kMean = 2 };
 // copy in padded rows.
 Tensor aligned_head(const Tensor& w) {
   const int64_t V = w.size(0), K = w.size(1);
-  if ((K == 1 || w.stride(1) == 1) && w.stride(0) % 8 == 0 && w.stride(0) >= K && (reinterpret_cast<uintptr_t>(ptr(w)) & 15) == 0)
+  if (!w.is_neg() && (K == 1 || w.stride(1) == 1) && w.stride(0) % 8 == 0 && w.stride(0) >= K && (reinterpret_cast<uintptr_t>(ptr(w)) & 15) == 0)
     return w.detach();
   Tensor out = empty(w, {V, (K + 7) / 8 * 8}, at::kBFloat16).narrow(1, 0, K);
   out.copy_(w.detach());
@@ -464,7 +468,7 @@ struct LinearCe : torch::autograd::Function<LinearCe> {
     const Tensor &w_ = kept[0], &saved = kept[1];
     const auto call = ctx->saved_data["call"].toIntVector();
     const int64_t T = call[0], K = call[1], V = w_.size(0), Kp = (K + 7) / 8 * 8, piece = call[3];
-    const Tensor w = aligned_head(w_), g = grads[0].reshape(-1);
+    const Tensor w = aligned_head(w_), g = plain(grads[0]).reshape(-1);
     const int sms = num_sms(w.device());
     const Launch on(w);
     const int64_t room = lib.b200_lce_backward_bytes((int)T, (int)V, (int)K, (int)Kp, (int)piece, (int)call[4], (int)call[5], sms);
@@ -513,7 +517,7 @@ Maybe linear_cross_entropy(const Tensor& h, const Tensor& w, const Tensor& targe
     const Tensor zero = h.to(at::kFloat).sum() + w.narrow(0, 0, 0).to(at::kFloat).sum();
     return reduction == kEach ? zero.expand(targets.sizes()) : zero;
   }
-  const Tensor h2 = rows2d(h, K), t1 = targets.reshape(-1).contiguous();
+  const Tensor h2 = rows2d(h, K), t1 = plain(targets).reshape(-1).contiguous();
   Tensor out;
   if (at::GradMode::is_enabled() && (h.requires_grad() || w.requires_grad())) {
     capturable("linear_cross_entropy", {h, w});
