@@ -175,6 +175,14 @@ void once(const char* what, const variable_list& grads) {
   for (const Tensor& g : grads) computable(what, {g});
 }
 
+// What autograd gives back of a saved tensor, which hooks of the caller may have replaced: the
+// kernels read it by the sizes, type and device that it had.
+Tensor kept(const char* what, const Tensor& t, const at::Device& device, at::ScalarType type, at::IntArrayRef sizes) {
+  TORCH_CHECK(t.defined() && t.device() == device && t.scalar_type() == type && t.sizes() == sizes, what,
+              ": a saved tensor came back changed");
+  return t;
+}
+
 // ------------------------------------------------------------------ dropout
 Tensor dropout_run(const Tensor& x, int64_t cut, uint64_t seed, uint64_t offset, const Tensor& offset_t, const Tensor& residual) {
   if (cut == 65536)  // nothing stays
@@ -304,21 +312,32 @@ struct BlockNorms : torch::autograd::Function<BlockNorms> {
     auto [y, h, r1, r2] = norms_run(x, delta, post, pre, gate, {kind, eps, scale, offset_one, round_branch}, Tensor(), true);
     ctx->save_for_backward({y, delta, post, pre, gate, r1, r2});
     ctx->saved_data["call"] = std::vector<int64_t>{kind, offset_one, wants_grad(x), wants_grad(delta), wants_grad(post),
-                                                   wants_grad(pre), wants_grad(gate)};
+                                                   wants_grad(pre), wants_grad(gate), post.defined(), pre.defined(),
+                                                   (int64_t)(post.defined() ? post : pre.defined() ? pre : x).scalar_type()};
     ctx->saved_data["scale"] = scale;
+    if (gate.defined()) ctx->saved_data["gate"] = gate.sizes().vec();
     if (h.defined()) return {y, h};
     return {y};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     once("block_norms", grads);
     const auto saved = ctx->get_saved_variables();
-    const Tensor &y = saved[0], &delta = saved[1], &post = saved[2], &pre = saved[3], &gate = saved[4], &r1 = saved[5],
-                 &r2 = saved[6];
     const auto call = ctx->saved_data["call"].toIntVector();
-    const int64_t kind = call[0], H = y.size(-1);
     const Tensor dy = grads[0], dh = grads.size() > 1 ? grads[1] : Tensor();
     variable_list out(10);
     if (!dy.defined() && !dh.defined()) return out;
+    // the engine has given either gradient y's sizes, type and device
+    const Tensor& like = dy.defined() ? dy : dh;
+    const int64_t kind = call[0], H = like.size(-1), rows = like.numel() / H;
+    auto back = [&](int i, at::ScalarType type, at::IntArrayRef sizes) {
+      return kept("block_norms", saved[i], like.device(), type, sizes);
+    };
+    const auto w_type = (at::ScalarType)call[9];
+    const Tensor y = back(0, like.scalar_type(), like.sizes()), delta = back(1, like.scalar_type(), like.sizes());
+    const Tensor post = call[7] ? back(2, w_type, {H}) : Tensor(), pre = call[8] ? back(3, w_type, {H}) : Tensor();
+    const Tensor gate = kind != kNone ? back(4, like.scalar_type(), ctx->saved_data["gate"].toIntVector()) : Tensor();
+    const Tensor r1 = call[7] ? back(5, at::kFloat, {rows}).contiguous() : Tensor();
+    const Tensor r2 = call[8] ? back(6, at::kFloat, {rows}).contiguous() : Tensor();
     Tensor &dx = out[0], &dd = out[1], &dpost = out[2], &dpre = out[3], &dgate = out[4];
     if (call[2]) dx = packed_like(y);
     if (call[3]) dd = packed_like(delta);
@@ -426,7 +445,8 @@ enum Reduction { kEach = 0, kSum = 1, kMean = 2 };
 // copy in padded rows.
 Tensor aligned_head(const Tensor& w) {
   const int64_t V = w.size(0), K = w.size(1);
-  if (!w.is_neg() && (K == 1 || w.stride(1) == 1) && w.stride(0) % 8 == 0 && w.stride(0) >= K && (reinterpret_cast<uintptr_t>(ptr(w)) & 15) == 0)
+  if (!w.is_neg() && (K == 1 || w.stride(1) == 1) && w.stride(0) % 8 == 0 && w.stride(0) >= K &&
+      (reinterpret_cast<uintptr_t>(ptr(w)) & 15) == 0)
     return w.detach();
   Tensor out = empty(w, {V, (K + 7) / 8 * 8}, at::kBFloat16).narrow(1, 0, K);
   out.copy_(w.detach());
@@ -458,16 +478,19 @@ struct LinearCe : torch::autograd::Function<LinearCe> {
     const CeOut r = ce_forward(h2, w, targets, cap, ignore, reduction);
     ctx->save_for_backward({w, r.saved});
     ctx->saved_data["call"] =
-        std::vector<int64_t>{h2.size(0), h2.size(1), reduction, piece, wants_grad(h2), wants_grad(w)};
+        std::vector<int64_t>{h2.size(0), h2.size(1), reduction, piece, wants_grad(h2), wants_grad(w), w.size(0)};
     ctx->saved_data["cap"] = cap;
     return r.out;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     once("linear_cross_entropy", grads);
-    const auto kept = ctx->get_saved_variables();
-    const Tensor &w_ = kept[0], &saved = kept[1];
     const auto call = ctx->saved_data["call"].toIntVector();
-    const int64_t T = call[0], K = call[1], V = w_.size(0), Kp = (K + 7) / 8 * 8, piece = call[3];
+    const int64_t T = call[0], K = call[1], V = call[6], Kp = (K + 7) / 8 * 8, piece = call[3];
+    const auto back = ctx->get_saved_variables();
+    const at::Device device = grads[0].device();
+    const Tensor w_ = kept("linear_cross_entropy", back[0], device, at::kBFloat16, {V, K});
+    const Tensor saved =
+        kept("linear_cross_entropy", back[1], device, at::kByte, {lib.b200_lce_saved_bytes((int)T, (int)Kp)}).contiguous();
     const Tensor w = aligned_head(w_), g = plain(grads[0]).reshape(-1);
     const int sms = num_sms(w.device());
     const Launch on(w);
