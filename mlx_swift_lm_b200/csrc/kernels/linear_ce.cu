@@ -103,7 +103,8 @@ static_assert(kSmem <= 227 * 1024, "shared memory plan exceeds the per-CTA limit
 // (a full step of 4096 rows 14.9 ms in one chunk, 15.5 as it is, 15.8 with 512 for both).
 template <int OP>
 constexpr int kChunk = OP == 0 ? 8 : OP == 1 ? 16 : 1 << 30;  // kStats, kGrad; the others' results are rounded to bf16
-// Those threads need more registers than 168, the share of 384: the other four warps give some of theirs.
+// Those threads need more registers than 168, the share of 384: the other four warps give some of
+// theirs (what is left to spill are 28 - 32 bytes a thread).
 constexpr int kRegsMax = 168, kRegsRest = 56, kRegsEpi = 224;
 static_assert(128 * kRegsRest + 256 * kRegsEpi <= kThreads * kRegsMax, "more registers than the block is launched with");
 
